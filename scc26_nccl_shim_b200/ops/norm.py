@@ -1,0 +1,285 @@
+"""Root-mean-square norm of a sum: what follows an AllReduce of activations.
+
+The partial sums of a row-parallel product (one tensor per rank, 1 to 8 of
+them) and the residual are added and normalised in one pass, with the result
+in the input's type or in e4m3 with scales; and the gradient of that.
+
+The kernels run on the current stream of the tensors' device, whichever device
+is current, and can be captured into a CUDA graph. Gradients are computed by
+an explicit call; nothing here is recorded by autograd.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import functools
+import math
+import struct
+from typing import NamedTuple, Sequence
+
+import torch
+
+from . import emu
+
+# ncclDataType_t
+DTYPE = {torch.float16: 6, torch.float32: 7, torch.bfloat16: 9}
+E4M3 = torch.float8_e4m3fn
+NCCL_E4M3 = 10
+GROUPS = (0, 32, 64, 128)
+
+_FWD = struct.Struct("8Q8q8qQ2q5Q2q7if")       # nb_norm_t
+_BWD = struct.Struct("Q2qQ2qQ2qQQQQQQ2q4i")    # nb_norm_grad_t
+_ERR = 256
+
+
+class NormOut(NamedTuple):
+    """What add_rms_norm returns. `y` is the normalised sum; `scale` holds the
+    scales of an e4m3 `y` (else None): y's value is y * scale of its group;
+    `h` is the sum (the next residual); `rstd` is 1 / rms of each row, which the
+    gradient needs."""
+    y: torch.Tensor
+    scale: torch.Tensor | None
+    h: torch.Tensor
+    rstd: torch.Tensor
+
+
+@functools.lru_cache(maxsize=1)
+def lib() -> C.CDLL:
+    L = emu.lib()
+    for f in (L.nb_add_rms_norm, L.nb_add_rms_norm_backward):
+        f.argtypes = [C.c_char_p, C.c_void_p, C.c_char_p, C.c_size_t]
+    L.nb_add_rms_norm_backward_workspace.argtypes = [C.c_int, C.c_int64, C.c_int]
+    L.nb_add_rms_norm_backward_workspace.restype = C.c_uint64
+    return L
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device: int, rows: int, hidden: int) -> int:
+    return int(lib().nb_add_rms_norm_backward_workspace(device, rows, hidden))
+
+
+def _strides(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(inner, outer stride, inner stride): row r of `t` starts at
+    (r // inner) * outer stride + (r % inner) * inner stride elements."""
+    hidden = t.shape[-1]
+    if t.is_contiguous():
+        return 1, hidden, 0
+    if t.stride(-1) != 1 and hidden > 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    dims: list[list[int]] = []  # [size, stride], neighbours merged
+    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+        if n == 1:
+            continue
+        if dims and dims[-1][1] == n * s:
+            dims[-1] = [dims[-1][0] * n, s]
+        else:
+            dims.append([n, s])
+    if not dims:
+        return 1, hidden, 0
+    if len(dims) == 1:
+        return 1, dims[0][1], 0
+    if len(dims) == 2:
+        return dims[1][0], dims[0][1], dims[1][1]
+    raise ValueError(f"{name}: rows at more than two different strides (call .contiguous())")
+
+
+def _rows(ts: Sequence[tuple[torch.Tensor, str]]) -> tuple[int, list[tuple[int, int]]]:
+    """The split of the row number that all of these share, and their strides."""
+    got = [_strides(t, name) for t, name in ts]
+    inner = 1
+    for (n, _, _), (_, name) in zip(got, ts):
+        if n != 1:
+            if inner != 1 and inner != n:
+                raise ValueError(f"{name}: rows are split unlike the other tensors' (call .contiguous())")
+            inner = n
+    if inner == 1:
+        return 1, [(o, i) for _, o, i in got]
+    return inner, [(o, i) if n != 1 else (inner * o, o) for n, o, i in got]
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _disjoint(a: torch.Tensor, b: torch.Tensor) -> bool:
+    if not a.numel() or not b.numel():
+        return True
+    (s, e), (p, q) = _span(a), _span(b)
+    return e <= p or q <= s
+
+
+def _check_weight(weight: torch.Tensor, hidden: int, dtype: torch.dtype, device: torch.device) -> None:
+    if weight.dim() != 1 or weight.shape[0] != hidden:
+        raise ValueError(f"weight: expected shape ({hidden},), got {tuple(weight.shape)}")
+    if weight.dtype != dtype and weight.dtype != torch.float32:
+        raise TypeError(f"weight: expected {dtype} or torch.float32, got {weight.dtype}")
+    if weight.stride(0) != 1 and hidden > 1:
+        raise ValueError("weight: must be contiguous")
+    if weight.device != device:
+        raise ValueError(f"weight: on {weight.device}, the input on {device}")
+
+
+def _like(t: torch.Tensor, ref: torch.Tensor, name: str) -> None:
+    if t.dtype != ref.dtype:
+        raise TypeError(f"{name}: expected {ref.dtype}, got {t.dtype}")
+    if t.shape != ref.shape:
+        raise ValueError(f"{name}: expected shape {tuple(ref.shape)}, got {tuple(t.shape)}")
+    if t.device != ref.device:
+        raise ValueError(f"{name}: on {t.device}, expected {ref.device}")
+
+
+def _on_gpu(t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise ValueError(f"the tensors must be on a CUDA device, got {t.device}")
+    return t.device.index
+
+
+def _stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _run(fn, packed: bytes, device: int) -> None:
+    err = C.create_string_buffer(_ERR)
+    rc = fn(packed, _stream(device), err, _ERR)
+    if rc:
+        raise RuntimeError(f"{err.value.decode()} ({rc})")
+
+
+def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6,
+                 out_dtype: torch.dtype | None = None, group: int = 0, out: NormOut | None = None) -> NormOut:
+    """h = x_0 + ... + x_{n-1} + residual; y = h / sqrt(mean(h^2) + eps) * weight.
+
+    `x` is a tensor [..., hidden] or a sequence of 1 to 8 of them (the partial
+    sums, added in order in fp32); fp16, bf16 or fp32, rows at up to two
+    strides. `weight` [hidden] has x's type or fp32. y is computed from the fp32
+    sum and rounded once; `h` is the sum rounded to x's type. A single x without
+    a residual comes back as `h` itself.
+
+    `out_dtype=torch.float8_e4m3fn`: y in e4m3, round to nearest even, with fp32
+    scales [..., ceil(hidden / group)] (`group` 32, 64 or 128 columns) or
+    [..., 1] (`group` 0: one per row); scale = max(largest magnitude / 448,
+    2^-126). A NaN makes its group's scale NaN.
+
+    Squares are summed in fp32: rows beyond about 1e19 overflow to y = 0.
+
+    `out` gives the outputs' memory (contiguous; `out.h` may be the residual or
+    x_0 itself, nothing else may overlap).
+    """
+    xs = [x] if isinstance(x, torch.Tensor) else list(x)
+    if not 1 <= len(xs) <= 8:
+        raise ValueError(f"1 to 8 partial sums, got {len(xs)}")
+    x0 = xs[0]
+    dtype, shape = x0.dtype, x0.shape
+    if dtype not in DTYPE:
+        raise TypeError(f"x: expected fp16, bf16 or fp32, got {dtype}")
+    if x0.dim() < 1 or shape[-1] < 1:
+        raise ValueError(f"x: expected shape [..., hidden] with hidden >= 1, got {tuple(shape)}")
+    hidden = shape[-1]
+    for i in range(1, len(xs)):
+        _like(xs[i], x0, f"x[{i}]")
+    if residual is not None:
+        _like(residual, x0, "residual")
+    _check_weight(weight, hidden, dtype, x0.device)
+    f8 = out_dtype == E4M3
+    if not f8 and out_dtype is not None and out_dtype != dtype:
+        raise TypeError(f"out_dtype: expected {dtype} or {E4M3}, got {out_dtype}")
+    if group not in GROUPS or (group and not f8):
+        raise ValueError(f"group: one of {GROUPS} with e4m3 output, else 0, got {group}")
+    if not 0 < eps < math.inf:
+        raise ValueError(f"eps: must be positive, got {eps}")
+    if out is None and residual is None and len(xs) == 1 and x0.is_contiguous():
+        inner, strides = 1, [(hidden, 0)]
+    else:
+        named = [(t, f"x[{i}]") for i, t in enumerate(xs)]
+        if residual is not None:
+            named.append((residual, "residual"))
+        inner, strides = _rows(named)
+    lead = shape[:-1]
+    sums = len(xs) > 1 or residual is not None
+    groups = -(-hidden // group) if group else 1
+    ydtype = E4M3 if f8 else dtype
+    if out is not None:
+        y, scale, h, rstd = _check_out(out, xs, weight, residual, ydtype, lead + (groups,) if f8 else None)
+    device = _on_gpu(x0)
+    if out is None:
+        y = torch.empty(shape, dtype=ydtype, device=x0.device)
+        scale = torch.empty(lead + (groups,), dtype=torch.float32, device=x0.device) if f8 else None
+        h = torch.empty(shape, dtype=dtype, device=x0.device) if sums else x0
+        rstd = torch.empty(lead, dtype=torch.float32, device=x0.device)
+    rows = rstd.numel()
+    pad = (0,) * (8 - len(xs))
+    ptrs = tuple([t.data_ptr() for t in xs]) + pad
+    outer = tuple([strides[i][0] for i in range(len(xs))]) + pad
+    inners = tuple([strides[i][1] for i in range(len(xs))]) + pad
+    r = (residual.data_ptr(), *strides[-1]) if residual is not None else (0, 0, 0)
+    _run(lib().nb_add_rms_norm,
+         _FWD.pack(*ptrs, *outer, *inners, *r, weight.data_ptr(), y.data_ptr(),
+                   scale.data_ptr() if f8 else 0, h.data_ptr() if h is not x0 or sums else 0, rstd.data_ptr(),
+                   rows, inner, device, hidden, len(xs), DTYPE[dtype], DTYPE[weight.dtype],
+                   NCCL_E4M3 if f8 else DTYPE[dtype], group, eps), device)
+    return NormOut(y, scale, h, rstd)
+
+
+def _check_out(out, xs, weight, residual, ydtype, scale_shape):
+    x0 = xs[0]
+    inputs = xs + [weight] + ([residual] if residual is not None else [])
+    want = [("y", out.y, x0.shape, ydtype), ("h", out.h, x0.shape, x0.dtype),
+            ("rstd", out.rstd, x0.shape[:-1], torch.float32)]
+    if scale_shape is not None:
+        want.append(("scale", out.scale, scale_shape, torch.float32))
+    elif out.scale is not None:
+        raise ValueError("out.scale: only an e4m3 output has scales")
+    for name, t, shape, dtype in want:
+        if t is None or t.shape != shape or t.dtype != dtype or t.device != x0.device:
+            raise ValueError(f"out.{name}: expected {tuple(shape)} of {dtype} on {x0.device}")
+    alone = len(xs) == 1 and residual is None
+    for i, (name, t, _, _) in enumerate(want):
+        same = [s for s in (xs[0], residual) if name == "h" and s is not None and
+                s.data_ptr() == t.data_ptr() and s.stride() == t.stride()]
+        if not t.is_contiguous():
+            raise ValueError(f"out.{name}: must be contiguous")
+        for other in inputs + [w[1] for w in want[i + 1:]]:
+            if not any(other is s for s in same) and not _disjoint(t, other):
+                raise ValueError(f"out.{name}: overlaps another tensor of the call")
+    if alone and out.h.data_ptr() == x0.data_ptr():
+        return out.y, out.scale, x0, out.rstd
+    return out.y, out.scale, out.h, out.rstd
+
+
+def add_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                          dh: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradient of add_rms_norm: (dx, dweight).
+
+    dx = rstd * (dy * w - n * mean(dy * w * n)) + dh with n = h * rstd is the
+    gradient of every partial sum and of the residual; `dh` is the gradient that
+    reaches the sum on its other way (the residual stream). dweight = sum over
+    rows of dy * n, in the weight's type, added in an order that depends on
+    the sizes alone. `h` and `rstd` are add_rms_norm's; dy, h and dh have one type.
+    """
+    if h.dtype not in DTYPE:
+        raise TypeError(f"h: expected fp16, bf16 or fp32, got {h.dtype}")
+    if h.dim() < 1 or h.shape[-1] < 1:
+        raise ValueError(f"h: expected shape [..., hidden] with hidden >= 1, got {tuple(h.shape)}")
+    hidden = h.shape[-1]
+    _like(dy, h, "dy")
+    if dh is not None:
+        _like(dh, h, "dh")
+    _check_weight(weight, hidden, h.dtype, h.device)
+    if rstd.dtype != torch.float32 or rstd.shape != h.shape[:-1] or not rstd.is_contiguous():
+        raise ValueError(f"rstd: expected {tuple(h.shape[:-1])} of torch.float32, contiguous")
+    if rstd.device != h.device:
+        raise ValueError(f"rstd: on {rstd.device}, expected {h.device}")
+    named = [(dy, "dy"), (h, "h")] + ([(dh, "dh")] if dh is not None else [])
+    inner, strides = _rows(named)
+    device = _on_gpu(h)
+    rows = rstd.numel()
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dw = torch.empty(hidden, dtype=weight.dtype, device=h.device)
+    nbytes = _workspace_bytes(device, rows, hidden)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=h.device)
+    s = (dh.data_ptr(), *strides[2]) if dh is not None else (0, 0, 0)
+    _run(lib().nb_add_rms_norm_backward,
+         _BWD.pack(dy.data_ptr(), *strides[0], h.data_ptr(), *strides[1], *s, weight.data_ptr(), rstd.data_ptr(),
+                   dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes, rows, inner, device, hidden,
+                   DTYPE[h.dtype], DTYPE[weight.dtype]), device)
+    return dx, dw

@@ -1,6 +1,7 @@
 // C entry points over the pure core, for the CPU test-suite (ctypes) and for
 // tools. Nothing here touches CUDA or NCCL; a fake GroupBackend stands in
 // for libnccl and the clique runner.
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -22,6 +23,7 @@
 #include "core/plan_sim.h"
 #include "core/policy.h"
 #include "core/summary.h"
+#include "core/tensor_table.h"
 
 using namespace nb;
 
@@ -660,6 +662,24 @@ int nb_classify_buffer(const nb_facts_t* first, const nb_facts_t* last, uint64_t
   const BufferVerdict v = classify_buffer(to_facts(*first), to_facts(*last), addr, bytes, device);
   copy_out(v.rule, rule, cap);
   return int(v.cls);
+}
+
+// The work list of a kernel over many tensors (tensor_table.h): the launches
+// for `launch` < 0, else that launch's tensors, first chunks and chunk count.
+int nb_pack_tensors(const uint64_t* sizes, size_t count, int room, int launch, int* tensor, unsigned* first,
+                    unsigned* chunks) {
+  const std::vector<TableLaunch> l = pack_tensors(sizes, count, room);
+  if (launch < 0) return int(l.size());
+  if (size_t(launch) >= l.size()) return -1;
+  const TableLaunch& t = l[size_t(launch)];
+  std::copy(t.tensor.begin(), t.tensor.end(), tensor);
+  std::copy(t.first.begin(), t.first.end(), first);
+  *chunks = t.chunks;
+  return int(t.tensor.size());
+}
+
+int nb_find_tensor(unsigned chunk, const unsigned* first, int count) {
+  return find_tensor(chunk, count, [&](int i) { return first[i]; });
 }
 
 }  // extern "C"

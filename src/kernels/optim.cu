@@ -1,0 +1,669 @@
+// AdamW and the gradients' norm over many tensors (see optim.h).
+//
+//   g = scale * (g_0 + ... + g_{n-1})                 (fp32, in order)
+//   m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// Bound by HBM: every array is read and written once (28 bytes an element
+// with fp32 parameters and states, a 16-bit gradient and a 16-bit copy; 16
+// with 8-bit states), so the arithmetic is plain fp32 in the order written.
+//
+// States in 8 bits. m and r = sqrt(v) are kept in e4m3, blocks of 256 (one
+// warp's eight elements per lane, so a block's maximum is one warp reduction)
+// with an fp32 scale that maps the block's largest magnitude to 448. r instead of v
+// halves the exponent range that the 8 bits have to cover. They are rounded
+// at random, to the neighbour below or above with the odds that keep the
+// mean: to nearest, a state that moves by less than half a step (3 to 6 %)
+// would never move, and beta2 = 0.999 moves v by 0.1 % a step. The random bits
+// are a hash of the seed, t, the tensor and the element, so a step is
+// reproducible. A positive r never rounds to zero, where m / (r + eps) would
+// explode. The update itself uses the unrounded m and v.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstring>
+#include <memory>
+#include <new>
+#include <vector>
+
+#include "core/tensor_table.h"
+#include "kernels/octet.cuh"
+#include "kernels/ophost.h"
+#include "kernels/optim.h"
+
+namespace nb {
+namespace {
+
+using namespace octet;
+
+constexpr int kThreads = 256;
+static_assert(kThreads * 8 == kChunk, "a chunk is eight elements per thread");
+static_assert(NB_OPTIM_BLOCK == 256, "a block is one warp's elements");
+
+// One tensor of the work list; its gradients' addresses follow the entries.
+struct Entry {
+  void* param;
+  void* copy;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  unsigned long long size;
+  unsigned first;  // its first chunk
+  unsigned index;  // its place in the caller's list
+  float decay;
+  int vec;         // every address is on an octet's boundary
+};
+constexpr int kEntryWords = sizeof(Entry) / 8;
+
+struct GradEntry {
+  unsigned long long size;
+  unsigned first;
+  int vec;
+};
+constexpr int kGradEntryWords = sizeof(GradEntry) / 8;
+
+// The list's room: few tensors keep the launch's parameters small.
+constexpr int kSmallWords = 448, kLargeWords = 4000;
+
+struct StepScalars {
+  const long long* t;
+  const float* lr;
+  const float* scale;
+  float t_lr_m;      // lr / (1 - b1^t), where both are the host's
+  float t_root;      // 1 / sqrt(1 - b2^t), where t is the host's
+  float lr_host, scale_host;
+  float inv1;        // 1 / (1 - b1^t), where t is the host's
+  unsigned t_host;
+};
+
+template <int WORDS>
+struct AdamArgs {
+  StepScalars s;
+  float b1, b1c, b2, b2c, eps, ln_b1, ln_b2;
+  unsigned seed, chunks;
+  int count, parts;
+  unsigned long long words[WORDS];
+};
+static_assert(sizeof(AdamArgs<kLargeWords>) <= 32764, "kernel parameters");
+static_assert(sizeof(AdamArgs<kSmallWords>) <= 4096, "kernel parameters");
+
+template <int WORDS>
+struct GradArgs {
+  double* partial;
+  unsigned chunks;
+  int count, parts;
+  unsigned long long words[WORDS];
+};
+
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0xA5CB9243u;
+  x ^= x >> 15;
+  x *= 0x5D8A37E5u;
+  return x ^ x >> 16;
+}
+
+// Rounds |z| <= 448 to e4m3 (as a float): down after u steps were added.
+__device__ __forceinline__ float round_random(float z, float u) {
+  int e = int(__float_as_uint(z) >> 23) - 130;  // log2 of the step between neighbours
+  e = e < -9 ? -9 : e;
+  const float step = __uint_as_float(uint32_t(e + 127) << 23), inv = __uint_as_float(uint32_t(127 - e) << 23);
+  return floorf(z * inv + u) * step;
+}
+
+// Where a lane's eight elements are: neighbours, or 32 apart so that single
+// elements coalesce. Both cover the warp's 256.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, unsigned long long warp_base, int lane, long long left, bool vec,
+                                      float (&f)[8]) {
+  if (vec) {
+    unpack<T>(load<T, true>(p + warp_base + lane * 8, 8), f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      f[j] = j * 32 + lane < left ? to_float<T>(p[warp_base + j * 32 + lane]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, unsigned long long warp_base, int lane, long long left, bool vec,
+                                       const float (&f)[8]) {
+  if (vec) {
+    store<T, true>(p + warp_base + lane * 8, f, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j * 32 + lane < left) p[warp_base + j * 32 + lane] = from_float<T>(f[j]);
+  }
+}
+
+__device__ __forceinline__ void load8_e4m3(const void* p, unsigned long long warp_base, int lane, long long left,
+                                           bool vec, float (&f)[8]) {
+  const uint8_t* b = static_cast<const uint8_t*>(p) + warp_base;
+  uint2 q = make_uint2(0, 0);
+  if (vec) {
+    q = *reinterpret_cast<const uint2*>(b + lane * 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t x = j * 32 + lane < left ? b[j * 32 + lane] : 0;
+      if (j < 4) q.x |= x << (8 * j);
+      else q.y |= x << (8 * (j - 4));
+    }
+  }
+  from_e4m3(q, f);
+}
+
+__device__ __forceinline__ void store8_e4m3(void* p, unsigned long long warp_base, int lane, long long left, bool vec,
+                                            const float (&f)[8]) {
+  uint8_t* b = static_cast<uint8_t*>(p) + warp_base;
+  const uint2 q = to_e4m3(f);
+  if (vec) {
+    *reinterpret_cast<uint2*>(b + lane * 8) = q;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j * 32 + lane < left) b[j * 32 + lane] = uint8_t((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+  }
+}
+
+// P: parameters; C: their copy (P itself: none); G: gradients; S8: states in e4m3.
+template <typename P, typename C, typename G, bool S8, int WORDS>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ AdamArgs<WORDS> a) {
+  constexpr bool kCopy = sizeof(C) != sizeof(P);
+  float scale = a.s.scale_host;
+  if (a.s.scale) scale *= *a.s.scale;
+  if (!(fabsf(scale) <= 3.4028235e38f)) return;  // no step
+  float lr = a.s.lr_host, root = a.s.t_root, size = a.s.t_lr_m;
+  unsigned t = a.s.t_host;
+  if (a.s.t || a.s.lr) {
+    if (a.s.lr) lr = *a.s.lr;
+    float inv1 = a.s.inv1;
+    if (a.s.t) {
+      // 1 - b^t = -expm1(t ln b): no cancellation while b^t is near 1.
+      const long long td = *a.s.t;
+      t = unsigned(td);
+      inv1 = 1.0f / -expm1f(float(td) * a.ln_b1);
+      root = 1.0f / sqrtf(-expm1f(float(td) * a.ln_b2));
+    }
+    size = lr * inv1;
+  }
+  const Entry* entries = reinterpret_cast<const Entry*>(a.words);
+  const unsigned long long* grads = a.words + (size_t)a.count * kEntryWords;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int i = find_tensor(blockIdx.x, a.count, [&](int k) { return entries[k].first; });
+  for (unsigned c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+    while (i + 1 < a.count && entries[i + 1].first <= c) ++i;
+    const Entry& e = entries[i];
+    const unsigned long long base = (unsigned long long)(c - e.first) * kChunk + (unsigned)warp * 256u;
+    if (base >= e.size) continue;  // the whole warp
+    const long long left = (long long)(e.size - base);
+    const bool vec = e.vec && left >= 256;
+    float g[8], m[8], v[8], p[8];
+    load8<P>(static_cast<const P*>(e.param), base, lane, left, vec, p);
+    float ms = 0.0f, vs = 0.0f;
+    if constexpr (S8) {
+      ms = e.m_scale[base >> 8];
+      vs = e.v_scale[base >> 8];
+      load8_e4m3(e.m, base, lane, left, vec, m);
+      load8_e4m3(e.v, base, lane, left, vec, v);
+    } else {
+      load8<float>(static_cast<const float*>(e.m), base, lane, left, vec, m);
+      load8<float>(static_cast<const float*>(e.v), base, lane, left, vec, v);
+    }
+    load8<G>(reinterpret_cast<const G*>(grads[(size_t)i * a.parts]), base, lane, left, vec, g);
+#pragma unroll 1
+    for (int k = 1; k < a.parts; ++k) {
+      float f[8];
+      load8<G>(reinterpret_cast<const G*>(grads[(size_t)i * a.parts + k]), base, lane, left, vec, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] += f[j];
+    }
+    const float keep = 1.0f - lr * e.decay;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      g[j] *= scale;
+      if constexpr (S8) {
+        m[j] *= ms;
+        v[j] *= vs;
+        v[j] *= v[j];
+      }
+      m[j] = m[j] * a.b1 + g[j] * a.b1c;
+      v[j] = v[j] * a.b2 + g[j] * g[j] * a.b2c;
+      const float r = sqrtf(v[j]);
+      p[j] = p[j] * keep - m[j] * size / (r * root + a.eps);
+      if constexpr (S8) v[j] = r;
+    }
+    store8<P>(static_cast<P*>(e.param), base, lane, left, vec, p);
+    if constexpr (kCopy) store8<C>(static_cast<C*>(e.copy), base, lane, left, vec, p);
+    if constexpr (!S8) {
+      store8<float>(static_cast<float*>(e.m), base, lane, left, vec, m);
+      store8<float>(static_cast<float*>(e.v), base, lane, left, vec, v);
+    } else {
+      uint32_t mt = 0, vt = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        mt = max(mt, magnitude(m[j]));
+        vt = max(vt, magnitude(v[j]));
+      }
+      ms = scale_of(__reduce_max_sync(~0u, mt));
+      vs = scale_of(__reduce_max_sync(~0u, vt));
+      const float mi = 1.0f / ms, vi = 1.0f / vs;
+      const uint32_t key = a.seed + t * 0x165667B1u + e.index * 0x3C6EF35Fu + uint32_t(base >> 32) * 0x6A09E667u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t at = uint32_t(base) + (vec ? lane * 8 + j : j * 32 + lane);
+        const uint32_t bits = mix(at * 0x9E3779B9u + key);
+        const float z = fabsf(m[j]) * mi, y = v[j] * vi;
+        m[j] = copysignf(round_random(z > kE4m3Max ? kE4m3Max : z, float(bits >> 16) * 0x1p-16f), m[j]);
+        const float q = round_random(y > kE4m3Max ? kE4m3Max : y, float(bits & 0xffffu) * 0x1p-16f);
+        v[j] = v[j] > 0.0f && q < 0x1p-9f ? 0x1p-9f : q;
+      }
+      store8_e4m3(e.m, base, lane, left, vec, m);
+      store8_e4m3(e.v, base, lane, left, vec, v);
+      if (lane == 0) {
+        e.m_scale[base >> 8] = ms;
+        e.v_scale[base >> 8] = vs;
+      }
+    }
+  }
+}
+
+// The sum of two doubles over a warp, in a fixed order.
+__device__ __forceinline__ double warp_sum(double s) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  return s;
+}
+
+// Squares of eight elements are added in fp32 and those sums in fp64: the
+// result does not depend on how many elements there are.
+template <typename G, int WORDS>
+__global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_constant__ GradArgs<WORDS> a) {
+  __shared__ double sums[kThreads / 32];
+  const GradEntry* entries = reinterpret_cast<const GradEntry*>(a.words);
+  const unsigned long long* grads = a.words + (size_t)a.count * kGradEntryWords;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double total = 0.0;
+  int i = find_tensor(blockIdx.x, a.count, [&](int k) { return entries[k].first; });
+  for (unsigned c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+    while (i + 1 < a.count && entries[i + 1].first <= c) ++i;
+    const GradEntry& e = entries[i];
+    const unsigned long long base = (unsigned long long)(c - e.first) * kChunk + (unsigned)warp * 256u;
+    if (base >= e.size) continue;
+    const long long left = (long long)(e.size - base);
+    const bool vec = e.vec && left >= 256;
+    float g[8], s = 0.0f;
+    load8<G>(reinterpret_cast<const G*>(grads[(size_t)i * a.parts]), base, lane, left, vec, g);
+#pragma unroll 1
+    for (int k = 1; k < a.parts; ++k) {
+      float f[8];
+      load8<G>(reinterpret_cast<const G*>(grads[(size_t)i * a.parts + k]), base, lane, left, vec, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] += f[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(g[j], g[j], s);
+    total += double(s);
+  }
+  total = warp_sum(total);
+  if (lane == 0) sums[warp] = total;
+  __syncthreads();
+  if (warp == 0) {
+    total = warp_sum(lane < kThreads / 32 ? sums[lane] : 0.0);
+    if (lane == 0) a.partial[blockIdx.x] = total;
+  }
+}
+
+__global__ void __launch_bounds__(1024) grad_norm_end_kernel(const double* partial, int count, double max_norm,
+                                                             double scale, float* out) {
+  __shared__ double sums[32];
+  double s = 0.0;
+  for (int k = threadIdx.x; k < count; k += 1024) s += partial[k];
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warp_sum(sums[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      const double norm = scale * sqrt(s);
+      const float shown = float(norm);
+      const double clip = max_norm / (norm + 1e-6);
+      out[0] = shown;
+      out[1] = fabsf(shown) <= 3.4028235e38f ? float(scale * (clip < 1.0 ? clip : 1.0)) : __int_as_float(0x7fffffff);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+int size_of(int dtype) {
+  switch (dtype) {
+    case NB_OPTIM_FLOAT16:
+    case NB_OPTIM_BFLOAT16: return 2;
+    case NB_OPTIM_FLOAT32: return 4;
+    default: return 0;
+  }
+}
+
+bool on_boundary(const void* p, size_t unit) { return reinterpret_cast<uintptr_t>(p) % unit == 0; }
+
+template <typename P, typename C, int WORDS>
+const void* adamw_by_grad(int grad, bool s8) {
+  switch (grad) {
+    case NB_OPTIM_FLOAT16:
+      return s8 ? reinterpret_cast<const void*>(adamw_kernel<P, C, __half, true, WORDS>)
+                : reinterpret_cast<const void*>(adamw_kernel<P, C, __half, false, WORDS>);
+    case NB_OPTIM_BFLOAT16:
+      return s8 ? reinterpret_cast<const void*>(adamw_kernel<P, C, __nv_bfloat16, true, WORDS>)
+                : reinterpret_cast<const void*>(adamw_kernel<P, C, __nv_bfloat16, false, WORDS>);
+    default:
+      return s8 ? reinterpret_cast<const void*>(adamw_kernel<P, C, float, true, WORDS>)
+                : reinterpret_cast<const void*>(adamw_kernel<P, C, float, false, WORDS>);
+  }
+}
+
+template <int WORDS>
+const void* adamw_for(int param, int copy, int grad, bool s8) {
+  if (param == NB_OPTIM_FLOAT16) return adamw_by_grad<__half, __half, WORDS>(grad, s8);
+  if (param == NB_OPTIM_BFLOAT16) return adamw_by_grad<__nv_bfloat16, __nv_bfloat16, WORDS>(grad, s8);
+  if (copy == NB_OPTIM_FLOAT16) return adamw_by_grad<float, __half, WORDS>(grad, s8);
+  if (copy == NB_OPTIM_BFLOAT16) return adamw_by_grad<float, __nv_bfloat16, WORDS>(grad, s8);
+  return adamw_by_grad<float, float, WORDS>(grad, s8);
+}
+
+template <int WORDS>
+const void* grad_norm_for(int grad) {
+  switch (grad) {
+    case NB_OPTIM_FLOAT16: return reinterpret_cast<const void*>(grad_norm_kernel<__half, WORDS>);
+    case NB_OPTIM_BFLOAT16: return reinterpret_cast<const void*>(grad_norm_kernel<__nv_bfloat16, WORDS>);
+    default: return reinterpret_cast<const void*>(grad_norm_kernel<float, WORDS>);
+  }
+}
+
+constexpr uint32_t kAdamMagic = 0x6164616d, kNormMagic = 0x6e6f726d;
+
+struct Launch {
+  bool large = false;
+  unsigned blocks = 0;
+  std::vector<unsigned long long> words;
+  unsigned chunks = 0;
+  int count = 0;
+};
+
+struct AdamHandle {
+  uint32_t magic = kAdamMagic;
+  int device = 0, parts = 1;
+  double beta1 = 0, beta2 = 0, eps = 0;
+  unsigned seed = 0;
+  const void* kernel[2] = {};  // small and large list
+  std::vector<Launch> launches;
+};
+
+struct NormHandle {
+  uint32_t magic = kNormMagic;
+  int device = 0, parts = 1, partials = 0;
+  const void* kernel[2] = {};
+  std::vector<Launch> launches;
+};
+
+template <typename E, typename Fill>
+std::vector<Launch> build_launches(const uint64_t* sizes, int count, int parts, const void* const* grad, int sms,
+                                   Fill fill) {
+  constexpr int kWords = sizeof(E) / 8;
+  std::vector<Launch> out;
+  for (const TableLaunch& t : pack_tensors(sizes, size_t(count), kLargeWords / (kWords + parts))) {
+    Launch l;
+    l.count = int(t.tensor.size());
+    l.chunks = t.chunks;
+    l.words.resize(size_t(l.count) * size_t(kWords + parts));
+    for (int k = 0; k < l.count; ++k) {
+      E e{};
+      const int i = t.tensor[size_t(k)];
+      e.size = sizes[i];
+      e.first = t.first[size_t(k)];
+      fill(i, e);
+      std::memcpy(&l.words[size_t(k) * kWords], &e, sizeof e);
+      for (int p = 0; p < parts; ++p)
+        l.words[size_t(l.count) * kWords + size_t(k) * size_t(parts) + size_t(p)] =
+            reinterpret_cast<unsigned long long>(grad[size_t(i) * size_t(parts) + size_t(p)]);
+    }
+    l.large = l.words.size() > size_t(kSmallWords);
+    const unsigned fit = unsigned(sms) * (2048 / kThreads);
+    l.blocks = l.chunks < fit ? l.chunks : fit;
+    out.push_back(std::move(l));
+  }
+  return out;
+}
+
+template <typename Args>
+cudaError_t launch_list(const Launch& l, const void* kernel, Args& args, cudaStream_t stream) {
+  args.count = l.count;
+  args.chunks = l.chunks;
+  std::memcpy(args.words, l.words.data(), l.words.size() * 8);
+  void* argv[] = {&args};
+  return cudaLaunchKernel(kernel, dim3(l.blocks), dim3(kThreads), argv, 0, stream);
+}
+
+// Lists of one launch: null entries and alignment to the element.
+const char* check_list(const uint64_t* sizes, int count, int parts, const void* const* grad, int gs) {
+  for (int i = 0; i < count; ++i) {
+    if (!sizes[i]) continue;
+    for (int p = 0; p < parts; ++p) {
+      const void* g = grad[size_t(i) * size_t(parts) + size_t(p)];
+      if (!g || !on_boundary(g, size_t(gs))) return "bad arguments: null or misaligned gradient";
+    }
+  }
+  return nullptr;
+}
+
+}  // namespace
+}  // namespace nb
+
+using namespace nb;
+
+extern "C" void* nb_adamw_create(const nb_adamw_t* a, char* err, size_t errcap) {
+  op_message(err, errcap, "");
+  const auto refuse = [&](const char* why) -> void* {
+    op_message(err, errcap, why);
+    return nullptr;
+  };
+  if (!a || a->count < 1 || !a->size || !a->param || !a->grad || !a->m || !a->v || !a->weight_decay)
+    return refuse("bad arguments: null or empty list of tensors");
+  if (a->parts < 1 || a->parts > 8) return refuse("bad arguments: 1 to 8 partial gradients");
+  const int ps = size_of(a->param_dtype), gs = size_of(a->grad_dtype), cs = a->copy_dtype ? size_of(a->copy_dtype) : 0;
+  if (!ps || !gs) return refuse("bad arguments: parameters and gradients are ncclFloat16, ncclFloat32 or ncclBfloat16");
+  if (a->copy_dtype && (cs != 2 || ps != 4 || !a->copy))
+    return refuse("bad arguments: a copy is ncclFloat16 or ncclBfloat16 beside ncclFloat32 parameters");
+  const bool s8 = a->state_dtype == NB_OPTIM_FLOAT8E4M3;
+  if (!s8 && a->state_dtype != NB_OPTIM_FLOAT32)
+    return refuse("bad arguments: states are ncclFloat32 or ncclFloat8e4m3");
+  if (s8 && (!a->m_scale || !a->v_scale)) return refuse("bad arguments: 8-bit states need their scales");
+  if (!(a->beta1 >= 0 && a->beta1 < 1) || !(a->beta2 >= 0 && a->beta2 < 1) || !(a->eps > 0) || !std::isfinite(a->eps))
+    return refuse("bad arguments: 0 <= beta < 1 and eps > 0");
+  if (const char* why = check_list(a->size, a->count, a->parts, a->grad, gs)) return refuse(why);
+  for (int i = 0; i < a->count; ++i) {
+    if (!std::isfinite(a->weight_decay[i])) return refuse("bad arguments: weight_decay must be finite");
+    if (!a->size[i]) continue;
+    if (!a->param[i] || !on_boundary(a->param[i], size_t(ps)) || !a->m[i] || !a->v[i] ||
+        (!s8 && (!on_boundary(a->m[i], 4) || !on_boundary(a->v[i], 4))) ||
+        (cs && (!a->copy[i] || !on_boundary(a->copy[i], size_t(cs)))) ||
+        (s8 && (!a->m_scale[i] || !a->v_scale[i] || !on_boundary(a->m_scale[i], 4) || !on_boundary(a->v_scale[i], 4))))
+      return refuse("bad arguments: null or misaligned tensor");
+  }
+  OpDevice dev(a->device);
+  if (dev.error()) return refuse("cannot use the device");
+  try {
+    std::unique_ptr<AdamHandle> h(new AdamHandle);
+    h->device = a->device;
+    h->parts = a->parts;
+    h->beta1 = a->beta1;
+    h->beta2 = a->beta2;
+    h->eps = a->eps;
+    h->seed = a->seed * 0x27D4EB2Fu;
+    h->kernel[0] = adamw_for<kSmallWords>(a->param_dtype, a->copy_dtype, a->grad_dtype, s8);
+    h->kernel[1] = adamw_for<kLargeWords>(a->param_dtype, a->copy_dtype, a->grad_dtype, s8);
+    h->launches = build_launches<Entry>(a->size, a->count, a->parts, a->grad, dev.sms(), [&](int i, Entry& e) {
+      e.param = a->param[i];
+      e.copy = cs ? a->copy[i] : nullptr;
+      e.m = a->m[i];
+      e.v = a->v[i];
+      e.m_scale = s8 ? a->m_scale[i] : nullptr;
+      e.v_scale = s8 ? a->v_scale[i] : nullptr;
+      e.index = unsigned(i);
+      e.decay = a->weight_decay[i];
+      bool vec = on_boundary(e.param, size_t(ps) * 8) && (!cs || on_boundary(e.copy, size_t(cs) * 8)) &&
+                 on_boundary(e.m, s8 ? 8 : 32) && on_boundary(e.v, s8 ? 8 : 32);
+      for (int p = 0; p < a->parts; ++p)
+        vec = vec && on_boundary(a->grad[size_t(i) * size_t(a->parts) + size_t(p)], size_t(gs) * 8);
+      e.vec = vec;
+    });
+    return h.release();
+  } catch (...) {
+    return refuse("out of host memory");
+  }
+}
+
+extern "C" int nb_adamw_step(const void* handle, int64_t t, const int64_t* t_dev, double lr, const float* lr_dev,
+                             double scale, const float* scale_dev, void* stream, char* err, size_t errcap) {
+  op_message(err, errcap, "");
+  const AdamHandle* h = static_cast<const AdamHandle*>(handle);
+  if (!h || h->magic != kAdamMagic) return op_refuse(err, errcap, "bad arguments: not an AdamW handle");
+  if (!t_dev && t < 1) return op_refuse(err, errcap, "bad arguments: steps count from 1");
+  if (!lr_dev && !std::isfinite(lr)) return op_refuse(err, errcap, "bad arguments: lr must be finite");
+  if (!std::isfinite(scale)) return op_refuse(err, errcap, "bad arguments: scale must be finite");
+  OpDevice dev(h->device);
+  if (dev.error()) return op_refuse(err, errcap, "cannot use the device", int(dev.error()));
+  StepScalars s{};
+  s.t = reinterpret_cast<const long long*>(t_dev);
+  s.lr = lr_dev;
+  s.scale = scale_dev;
+  s.lr_host = float(lr);
+  s.scale_host = float(scale);
+  s.t_host = unsigned(t);
+  if (!t_dev) {
+    const double inv1 = 1.0 / -std::expm1(double(t) * std::log(h->beta1));
+    s.inv1 = float(inv1);
+    s.t_lr_m = float(lr * inv1);
+    s.t_root = float(1.0 / std::sqrt(-std::expm1(double(t) * std::log(h->beta2))));
+  }
+  const auto fill = [&](auto& k) {
+    k.s = s;
+    k.b1 = float(h->beta1);
+    k.b1c = float(1.0 - h->beta1);
+    k.b2 = float(h->beta2);
+    k.b2c = float(1.0 - h->beta2);
+    k.eps = float(h->eps);
+    k.ln_b1 = float(std::log(h->beta1));
+    k.ln_b2 = float(std::log(h->beta2));
+    k.seed = h->seed;
+    k.parts = h->parts;
+  };
+  for (const Launch& l : h->launches) {
+    cudaError_t e;
+    if (l.large) {
+      AdamArgs<kLargeWords> k;
+      fill(k);
+      e = launch_list(l, h->kernel[1], k, static_cast<cudaStream_t>(stream));
+    } else {
+      AdamArgs<kSmallWords> k;
+      fill(k);
+      e = launch_list(l, h->kernel[0], k, static_cast<cudaStream_t>(stream));
+    }
+    if (e != cudaSuccess) return op_refuse(err, errcap, "launch of the AdamW step failed", int(e));
+  }
+  return 0;
+}
+
+extern "C" void nb_adamw_destroy(void* handle) {
+  AdamHandle* h = static_cast<AdamHandle*>(handle);
+  if (h && h->magic == kAdamMagic) {
+    h->magic = 0;
+    delete h;
+  }
+}
+
+extern "C" void* nb_grad_norm_create(int device, int count, int parts, int dtype, const uint64_t* size,
+                                     const void* const* grad, char* err, size_t errcap) {
+  op_message(err, errcap, "");
+  const auto refuse = [&](const char* why) -> void* {
+    op_message(err, errcap, why);
+    return nullptr;
+  };
+  if (count < 1 || !size || !grad) return refuse("bad arguments: null or empty list of tensors");
+  if (parts < 1 || parts > 8) return refuse("bad arguments: 1 to 8 partial gradients");
+  const int gs = size_of(dtype);
+  if (!gs) return refuse("bad arguments: gradients are ncclFloat16, ncclFloat32 or ncclBfloat16");
+  if (const char* why = check_list(size, count, parts, grad, gs)) return refuse(why);
+  OpDevice dev(device);
+  if (dev.error()) return refuse("cannot use the device");
+  try {
+    std::unique_ptr<NormHandle> h(new NormHandle);
+    h->device = device;
+    h->parts = parts;
+    h->kernel[0] = grad_norm_for<kSmallWords>(dtype);
+    h->kernel[1] = grad_norm_for<kLargeWords>(dtype);
+    h->launches = build_launches<GradEntry>(size, count, parts, grad, dev.sms(), [&](int i, GradEntry& e) {
+      bool vec = true;
+      for (int p = 0; p < parts; ++p)
+        vec = vec && on_boundary(grad[size_t(i) * size_t(parts) + size_t(p)], size_t(gs) * 8);
+      e.vec = vec;
+    });
+    for (const Launch& l : h->launches) h->partials += int(l.blocks);
+    return h.release();
+  } catch (...) {
+    return refuse("out of host memory");
+  }
+}
+
+extern "C" int nb_grad_norm_partials(const void* handle) {
+  const NormHandle* h = static_cast<const NormHandle*>(handle);
+  return h && h->magic == kNormMagic ? h->partials : -1;
+}
+
+extern "C" int nb_grad_norm(const void* handle, double max_norm, double scale, float* out, double* workspace,
+                            void* stream, char* err, size_t errcap) {
+  op_message(err, errcap, "");
+  const NormHandle* h = static_cast<const NormHandle*>(handle);
+  if (!h || h->magic != kNormMagic) return op_refuse(err, errcap, "bad arguments: not a gradient norm's handle");
+  if (!(max_norm > 0)) return op_refuse(err, errcap, "bad arguments: max_norm must be positive");
+  if (!(scale > 0) || !std::isfinite(scale)) return op_refuse(err, errcap, "bad arguments: scale must be positive");
+  if (!out || !on_boundary(out, 4) || (h->partials && (!workspace || !on_boundary(workspace, 8))))
+    return op_refuse(err, errcap, "bad arguments: null or misaligned output or workspace");
+  OpDevice dev(h->device);
+  if (dev.error()) return op_refuse(err, errcap, "cannot use the device", int(dev.error()));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  double* at = workspace;
+  for (const Launch& l : h->launches) {
+    cudaError_t e;
+    if (l.large) {
+      GradArgs<kLargeWords> k;
+      k.partial = at;
+      k.parts = h->parts;
+      e = launch_list(l, h->kernel[1], k, st);
+    } else {
+      GradArgs<kSmallWords> k;
+      k.partial = at;
+      k.parts = h->parts;
+      e = launch_list(l, h->kernel[0], k, st);
+    }
+    if (e != cudaSuccess) return op_refuse(err, errcap, "launch of the gradient norm failed", int(e));
+    at += l.blocks;
+  }
+  const double* partial = workspace;
+  int count = h->partials;
+  double limit = max_norm;
+  void* argv[] = {&partial, &count, &limit, &scale, &out};
+  const cudaError_t e = cudaLaunchKernel(reinterpret_cast<const void*>(grad_norm_end_kernel), dim3(1), dim3(1024),
+                                         argv, 0, st);
+  return e == cudaSuccess ? 0 : op_refuse(err, errcap, "launch of the gradient norm failed", int(e));
+}
+
+extern "C" void nb_grad_norm_destroy(void* handle) {
+  NormHandle* h = static_cast<NormHandle*>(handle);
+  if (h && h->magic == kNormMagic) {
+    h->magic = 0;
+    delete h;
+  }
+}
