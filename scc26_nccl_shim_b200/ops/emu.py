@@ -43,6 +43,13 @@ def _stream(t):
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def raw_stream(device: int) -> int:
+    """The current stream of `device` as a cudaStream_t."""
+    import torch
+    fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # no Stream object is made
+    return fast(device) if fast else torch.cuda.current_stream(device).cuda_stream
+
+
 def reduce(srcs, dsts, op="sum", nranks=None, scalars=None, nbytes=None):
     t = srcs[0]
     dt = DTYPE[TORCH_TO_DTYPE[str(t.dtype)]]

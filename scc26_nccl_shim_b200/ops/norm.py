@@ -28,6 +28,7 @@ GROUPS = (0, 32, 64, 128)
 
 _FWD = struct.Struct("8Q8q8qQ2q5Q2q7if")       # nb_norm_t
 _BWD = struct.Struct("Q2qQ2qQ2qQQQQQQ2q4i")    # nb_norm_grad_t
+_PAD = [(0,) * (8 - n) for n in range(9)]
 _ERR = 256
 
 
@@ -47,14 +48,14 @@ def lib() -> C.CDLL:
     L = emu.lib()
     for f in (L.nb_add_rms_norm, L.nb_add_rms_norm_backward):
         f.argtypes = [C.c_char_p, C.c_void_p, C.c_char_p, C.c_size_t]
-    L.nb_add_rms_norm_backward_workspace.argtypes = [C.c_int, C.c_int64, C.c_int]
+    L.nb_add_rms_norm_backward_workspace.argtypes = [C.c_int, C.c_int64, C.c_int, C.c_int]
     L.nb_add_rms_norm_backward_workspace.restype = C.c_uint64
     return L
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(device: int, rows: int, hidden: int) -> int:
-    return int(lib().nb_add_rms_norm_backward_workspace(device, rows, hidden))
+def _workspace_bytes(device: int, rows: int, hidden: int, dtype: int) -> int:
+    return int(lib().nb_add_rms_norm_backward_workspace(device, rows, hidden, dtype))
 
 
 def _strides(t: torch.Tensor, name: str) -> tuple[int, int, int]:
@@ -84,6 +85,9 @@ def _strides(t: torch.Tensor, name: str) -> tuple[int, int, int]:
 
 def _rows(ts: Sequence[tuple[torch.Tensor, str]]) -> tuple[int, list[tuple[int, int]]]:
     """The split of the row number that all of these share, and their strides."""
+    hidden = ts[0][0].shape[-1]
+    if all([t.is_contiguous() for t, _ in ts]):
+        return 1, [(hidden, 0)] * len(ts)
     got = [_strides(t, name) for t, name in ts]
     inner = 1
     for (n, _, _), (_, name) in zip(got, ts):
@@ -134,15 +138,20 @@ def _on_gpu(t: torch.Tensor) -> int:
     return t.device.index
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _run(fn, packed: bytes, device: int) -> None:
     err = C.create_string_buffer(_ERR)
-    rc = fn(packed, _stream(device), err, _ERR)
+    rc = fn(packed, emu.raw_stream(device), err, _ERR)
     if rc:
         raise RuntimeError(f"{err.value.decode()} ({rc})")
+
+
+def _empty(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    # torch.empty takes more than twice as long to read its arguments.
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1] or 1, 1), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
 
 
 def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6,
@@ -187,13 +196,10 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
         raise ValueError(f"group: one of {GROUPS} with e4m3 output, else 0, got {group}")
     if not 0 < eps < math.inf:
         raise ValueError(f"eps: must be positive, got {eps}")
-    if out is None and residual is None and len(xs) == 1 and x0.is_contiguous():
-        inner, strides = 1, [(hidden, 0)]
-    else:
-        named = [(t, f"x[{i}]") for i, t in enumerate(xs)]
-        if residual is not None:
-            named.append((residual, "residual"))
-        inner, strides = _rows(named)
+    named = [(t, "x") for t in xs]
+    if residual is not None:
+        named.append((residual, "residual"))
+    inner, strides = _rows(named)
     lead = shape[:-1]
     sums = len(xs) > 1 or residual is not None
     groups = -(-hidden // group) if group else 1
@@ -202,20 +208,20 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
         y, scale, h, rstd = _check_out(out, xs, weight, residual, ydtype, lead + (groups,) if f8 else None)
     device = _on_gpu(x0)
     if out is None:
-        y = torch.empty(shape, dtype=ydtype, device=x0.device)
-        scale = torch.empty(lead + (groups,), dtype=torch.float32, device=x0.device) if f8 else None
-        h = torch.empty(shape, dtype=dtype, device=x0.device) if sums else x0
-        rstd = torch.empty(lead, dtype=torch.float32, device=x0.device)
+        dev = x0.device
+        y = _empty(shape, ydtype, dev)
+        scale = _empty(lead + (groups,), torch.float32, dev) if f8 else None
+        h = _empty(shape, dtype, dev) if sums else x0
+        rstd = _empty(lead, torch.float32, dev)
     rows = rstd.numel()
-    pad = (0,) * (8 - len(xs))
-    ptrs = tuple([t.data_ptr() for t in xs]) + pad
-    outer = tuple([strides[i][0] for i in range(len(xs))]) + pad
-    inners = tuple([strides[i][1] for i in range(len(xs))]) + pad
-    r = (residual.data_ptr(), *strides[-1]) if residual is not None else (0, 0, 0)
+    n = len(xs)
+    pad = _PAD[n]
+    r = (residual.data_ptr(), *strides[n]) if residual is not None else (0, 0, 0)
     _run(lib().nb_add_rms_norm,
-         _FWD.pack(*ptrs, *outer, *inners, *r, weight.data_ptr(), y.data_ptr(),
+         _FWD.pack(*[t.data_ptr() for t in xs], *pad, *[o for o, _ in strides[:n]], *pad,
+                   *[i for _, i in strides[:n]], *pad, *r, weight.data_ptr(), y.data_ptr(),
                    scale.data_ptr() if f8 else 0, h.data_ptr() if h is not x0 or sums else 0, rstd.data_ptr(),
-                   rows, inner, device, hidden, len(xs), DTYPE[dtype], DTYPE[weight.dtype],
+                   rows, inner, device, hidden, n, DTYPE[dtype], DTYPE[weight.dtype],
                    NCCL_E4M3 if f8 else DTYPE[dtype], group, eps), device)
     return NormOut(y, scale, h, rstd)
 
@@ -273,10 +279,10 @@ def add_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
     inner, strides = _rows(named)
     device = _on_gpu(h)
     rows = rstd.numel()
-    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    dw = torch.empty(hidden, dtype=weight.dtype, device=h.device)
-    nbytes = _workspace_bytes(device, rows, hidden)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=h.device)
+    dx = _empty(h.shape, h.dtype, h.device)
+    dw = _empty((hidden,), weight.dtype, h.device)
+    nbytes = _workspace_bytes(device, rows, hidden, DTYPE[h.dtype])
+    ws = _empty((nbytes // 4,), torch.float32, h.device)
     s = (dh.data_ptr(), *strides[2]) if dh is not None else (0, 0, 0)
     _run(lib().nb_add_rms_norm_backward,
          _BWD.pack(dy.data_ptr(), *strides[0], h.data_ptr(), *strides[1], *s, weight.data_ptr(), rstd.data_ptr(),

@@ -55,10 +55,6 @@ def lib() -> C.CDLL:
     return L
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _addresses(ts) -> C.Array:
     return (C.c_uint64 * len(ts))(*[t.data_ptr() for t in ts])
 
@@ -152,10 +148,10 @@ class GradNorm(_Bound):
         Where the norm is not finite the coefficient is NaN. The same inputs give
         the same bits."""
         self._check_storages()
-        out = torch.empty(2, dtype=torch.float32, device=self.device)
-        ws = torch.empty(self._partials, dtype=torch.float64, device=self.device)
+        out = torch.empty_strided((2,), (1,), dtype=torch.float32, device=self.device)
+        ws = torch.empty_strided((self._partials,), (1,), dtype=torch.float64, device=self.device)
         err = C.create_string_buffer(_ERR)
-        rc = lib().nb_grad_norm(self._handle, max_norm, scale, out.data_ptr(), ws.data_ptr(), _stream(self._index),
+        rc = lib().nb_grad_norm(self._handle, max_norm, scale, out.data_ptr(), ws.data_ptr(), emu.raw_stream(self._index),
                                 err, _ERR)
         if rc:
             raise (ValueError if rc == -1 else RuntimeError)(f"{err.value.decode()} ({rc})")
@@ -219,8 +215,8 @@ class AdamW(_Bound):
         if len(decay) != len(params) or not all(math.isfinite(w) for w in decay):
             raise ValueError("weight_decay: a finite number, or one per parameter")
         b1, b2 = betas
-        if not (0 <= b1 < 1 and 0 <= b2 < 1) or not 0 < eps < math.inf:
-            raise ValueError("betas must be in [0, 1) and eps positive")
+        if not (0 <= b1 < 1 and 0 <= b2 < 1) or not 1.2e-38 <= eps <= 3.4e38:
+            raise ValueError("betas must be in [0, 1) and eps a positive normal fp32 number")
         if state not in ("float32", "8bit"):
             raise ValueError(f'state: "float32" or "8bit", got {state!r}')
         self._eight = state == "8bit"
@@ -285,7 +281,7 @@ class AdamW(_Bound):
         lr, lr_dev = self._scalar(lr, "lr", torch.float32)
         scale, scale_dev = self._scalar(scale, "scale", torch.float32)
         err = C.create_string_buffer(_ERR)
-        rc = lib().nb_adamw_step(self._handle, t, t_dev, lr, lr_dev, scale, scale_dev, _stream(self._index), err, _ERR)
+        rc = lib().nb_adamw_step(self._handle, t, t_dev, lr, lr_dev, scale, scale_dev, emu.raw_stream(self._index), err, _ERR)
         if rc:
             raise (ValueError if rc == -1 else RuntimeError)(f"{err.value.decode()} ({rc})")
         if self._versions:

@@ -666,9 +666,9 @@ int nb_classify_buffer(const nb_facts_t* first, const nb_facts_t* last, uint64_t
 
 // The work list of a kernel over many tensors (tensor_table.h): the launches
 // for `launch` < 0, else that launch's tensors, first chunks and chunk count.
-int nb_pack_tensors(const uint64_t* sizes, size_t count, int room, int launch, int* tensor, unsigned* first,
+int nb_pack_tensors(const uint64_t* sizes, size_t count, int room, unsigned chunk, int launch, int* tensor, unsigned* first,
                     unsigned* chunks) {
-  const std::vector<TableLaunch> l = pack_tensors(sizes, count, room);
+  const std::vector<TableLaunch> l = pack_tensors(sizes, count, room, chunk);
   if (launch < 0) return int(l.size());
   if (size_t(launch) >= l.size()) return -1;
   const TableLaunch& t = l[size_t(launch)];

@@ -2,7 +2,7 @@
 // of it, each chunk of a launch covers. Shared by the kernels, the host that
 // packs the launches, and the CPU tests.
 //
-// A tensor of n elements is ceil(n / kChunk) chunks; a launch numbers the
+// A tensor of n elements is ceil(n / chunk) chunks; a launch numbers the
 // chunks of its tensors one after another. The list travels in the launch's
 // parameters (32764 bytes at most on sm_100), so a step needs no copy, no
 // device table that a captured graph could outlive, and no workspace; tensors
@@ -20,8 +20,6 @@
 #endif
 
 namespace nb {
-
-constexpr unsigned kChunk = 2048;  // elements per chunk: 256 threads x 8
 
 // The tensor of chunk `c`: the last of `count` whose first chunk is not above
 // it. `first(i)` gives tensor i's first chunk; first(0) is 0, and a tensor
@@ -46,6 +44,6 @@ struct TableLaunch {
 
 // Splits the tensors (in order, those without elements left out) into
 // launches of at most `room` tensors and fewer than 2^31 chunks.
-std::vector<TableLaunch> pack_tensors(const uint64_t* sizes, size_t count, int room);
+std::vector<TableLaunch> pack_tensors(const uint64_t* sizes, size_t count, int room, unsigned chunk);
 
 }  // namespace nb

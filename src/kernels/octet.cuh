@@ -2,9 +2,7 @@
 // over the threads of a row: shared by the norm and the optimizer kernels.
 //
 // An octet of a 16-bit type is one 16-byte access, of fp32 one 32-byte access
-// (ld/st.global.v8, sm_100). Where a pointer, a stride or a length keeps an
-// octet off that boundary the same eight elements move one by one, under the
-// bounds of their row.
+// (ld/st.global.v8, sm_100).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -20,6 +18,34 @@ constexpr float kE4m3Max = 448.0f;
 // The least scale of a group of 8-bit values (2^-126): its reciprocal is finite.
 constexpr float kLeastScale = 1.17549435e-38f;
 
+// Two fp32 operations in one instruction (sm_100), each rounded as usual.
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v));
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 template <typename T>
 struct Oct {
   uint4 v[sizeof(T) / 2];
@@ -34,81 +60,131 @@ __device__ __forceinline__ T from_float(float x) { return T(x); }
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// `left` elements from p on exist; the others read as zero. Plain (coherent)
-// loads: an output may be one of the inputs.
-template <typename T, bool VEC>
-__device__ __forceinline__ Oct<T> load(const T* p, int left) {
+template <typename T>
+__device__ __forceinline__ Oct<T> load_oct(const T* p) {
   Oct<T> o;
-  if constexpr (VEC) {
-    if constexpr (sizeof(T) == 4) {
-      asm volatile("ld.global.v8.u32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                   : "=r"(o.v[0].x), "=r"(o.v[0].y), "=r"(o.v[0].z), "=r"(o.v[0].w), "=r"(o.v[1].x),
-                     "=r"(o.v[1].y), "=r"(o.v[1].z), "=r"(o.v[1].w)
-                   : "l"(p));
-    } else {
-      asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(o.v[0].x), "=r"(o.v[0].y), "=r"(o.v[0].z), "=r"(o.v[0].w)
-                   : "l"(p));
-    }
+  if constexpr (sizeof(T) == 4) {
+    asm volatile("ld.global.v8.u32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(o.v[0].x), "=r"(o.v[0].y), "=r"(o.v[0].z), "=r"(o.v[0].w), "=r"(o.v[1].x), "=r"(o.v[1].y),
+                   "=r"(o.v[1].z), "=r"(o.v[1].w)
+                 : "l"(p));
   } else {
-    T e[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = j < left ? p[j] : from_float<T>(0.0f);
-    uint32_t* w = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        w[j] = __float_as_uint(e[j]);
-      } else {
-        const uint32_t b = *reinterpret_cast<const uint16_t*>(&e[j]);
-        w[j / 2] = j & 1 ? w[j / 2] | b << 16 : b;
-      }
-    }
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(o.v[0].x), "=r"(o.v[0].y), "=r"(o.v[0].z), "=r"(o.v[0].w)
+                 : "l"(p));
   }
   return o;
+}
+
+// Two neighbours of a 16-bit type at a time.
+__device__ __forceinline__ float2 to_float2(__half, uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 to_float2(__nv_bfloat16, uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t from_float2(__half, float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t from_float2(__nv_bfloat16, float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 template <typename T>
 __device__ __forceinline__ void unpack(const Oct<T>& o, float (&f)[8]) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(&o);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if constexpr (sizeof(T) == 4) {
-      f[j] = __uint_as_float(w[j]);
-    } else {
-      const uint16_t b = uint16_t(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
-      f[j] = to_float<T>(*reinterpret_cast<const T*>(&b));
+    for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 v = to_float2(T(), w[j]);
+      f[2 * j] = v.x;
+      f[2 * j + 1] = v.y;
     }
   }
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store(T* p, const float (&f)[8], int left) {
-  if constexpr (VEC) {
-    uint32_t w[sizeof(T) * 2];
+template <typename T>
+__device__ __forceinline__ void unpack(const Oct<T>& o, Pair (&p)[4]) {
+  float f[8];
+  unpack<T>(o, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (sizeof(T) == 4) {
-        w[j] = __float_as_uint(f[j]);
-      } else {
-        const T e = from_float<T>(f[j]);
-        const uint32_t b = *reinterpret_cast<const uint16_t*>(&e);
-        w[j / 2] = j & 1 ? w[j / 2] | b << 16 : b;
-      }
-    }
-    if constexpr (sizeof(T) == 4) {
-      asm volatile("st.global.v8.u32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
-                   "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                   : "memory");
-    } else {
-      asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                   "r"(w[3])
-                   : "memory");
-    }
+  for (int j = 0; j < 4; ++j) p[j] = pair(f[2 * j], f[2 * j + 1]);
+}
+
+__device__ __forceinline__ void split(const Pair (&p)[4], float (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) split(p[j], f[2 * j], f[2 * j + 1]);
+}
+
+template <typename T>
+__device__ __forceinline__ Oct<T> pack(const float (&f)[8]) {
+  Oct<T> o;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(f[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = from_float2(T(), f[2 * j], f[2 * j + 1]);
+  }
+  return o;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const Oct<T>& o) {
+  if constexpr (sizeof(T) == 4) {
+    asm volatile("st.global.v8.u32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(o.v[0].x), "r"(o.v[0].y),
+                 "r"(o.v[0].z), "r"(o.v[0].w), "r"(o.v[1].x), "r"(o.v[1].y), "r"(o.v[1].z), "r"(o.v[1].w)
+                 : "memory");
+  } else {
+    asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(o.v[0].x), "r"(o.v[0].y), "r"(o.v[0].z),
+                 "r"(o.v[0].w)
+                 : "memory");
+  }
+}
+
+// Eight elements of a row as they are loaded, and their way back. VEC: an
+// octet of neighbours on its boundary. Otherwise single elements `step` apart,
+// with the row's other threads between them, so that a warp's accesses are
+// neighbours (cutting unaligned octets out of aligned pieces took 92
+// instructions an element of a norm, single elements take a fifth of that).
+// `left`: elements of the row from the first on; those beyond read as zero.
+// Plain (coherent) loads: an output may be one of the inputs.
+template <typename T, bool VEC>
+struct Raw {
+  Oct<T> o;
+
+  __device__ __forceinline__ void load(const T* p, int, int) { o = load_oct(p); }
+  __device__ __forceinline__ void get(Pair (&f)[4]) const { unpack<T>(o, f); }
+};
+
+template <typename T>
+struct Raw<T, false> {
+  T e[8];
+
+  __device__ __forceinline__ void load(const T* p, int step, int left) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = j * step < left ? p[j * step] : from_float<T>(0.0f);
+  }
+  __device__ __forceinline__ void get(Pair (&f)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = pair(to_float<T>(e[2 * j]), to_float<T>(e[2 * j + 1]));
+  }
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8], int step, int left) {
+  if constexpr (VEC) {
+    if (left > 0) store_vec<T>(p, pack<T>(f));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < left) p[j] = from_float<T>(f[j]);
+      if (j * step < left) p[j * step] = from_float<T>(f[j]);
   }
 }
 
@@ -132,9 +208,30 @@ __device__ __forceinline__ void from_e4m3(uint2 q, float (&f)[8]) {
   }
 }
 
-// Magnitudes compare as their bit patterns do, and a NaN is above infinity:
-// an integer maximum keeps a NaN that fmaxf would drop.
+// The larger magnitude; NaN where one is (fmaxf would drop it). Magnitudes
+// compare as their bit patterns do, a NaN above infinity, so that maxima over
+// threads may be integer ones.
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t top_of(const float (&f)[8]) {
+  float m = fabsf(f[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) m = max_magnitude(m, f[j]);
+  return magnitude(m);
+}
+// The same of those that exist: eight of VEC's, or the ones below `left`.
+template <bool VEC>
+__device__ __forceinline__ uint32_t top_of(const float (&f)[8], int step, int left) {
+  if constexpr (VEC) return top_of(f);
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, j * step < left ? magnitude(f[j]) : 0);
+  return m;
+}
 
 // The scale of a group whose largest magnitude is `top`; NaN stays NaN.
 __device__ __forceinline__ float scale_of(uint32_t top) {

@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdio>
 
@@ -21,14 +22,21 @@ inline int op_refuse(char* err, size_t cap, const char* msg, int code = -1) {
 // Makes `device` current and restores the caller's device on exit.
 class OpDevice {
  public:
-  explicit OpDevice(int device) : device_(device) {
+  explicit OpDevice(int device) {
     err_ = cudaGetDevice(&before_);
     if (err_ == cudaSuccess && before_ != device) {
       err_ = cudaSetDevice(device);
       switched_ = err_ == cudaSuccess;
     }
-    if (err_ == cudaSuccess) err_ = cudaDeviceGetAttribute(&sms_, cudaDevAttrMultiProcessorCount, device_);
-    if (err_ == cudaSuccess && sms_ < 1) sms_ = 1;
+    // 0: no SM count known yet. Threads that race store the same number.
+    static std::atomic<int> known[64];
+    const bool keeps = device >= 0 && device < 64;
+    if (err_ == cudaSuccess && keeps) sms_ = known[device].load(std::memory_order_relaxed);
+    if (err_ == cudaSuccess && !sms_) {
+      err_ = cudaDeviceGetAttribute(&sms_, cudaDevAttrMultiProcessorCount, device);
+      if (err_ == cudaSuccess && sms_ < 1) sms_ = 1;
+      if (err_ == cudaSuccess && keeps) known[device].store(sms_, std::memory_order_relaxed);
+    }
   }
   ~OpDevice() {
     if (switched_) cudaSetDevice(before_);
@@ -40,7 +48,7 @@ class OpDevice {
 
  private:
   cudaError_t err_ = cudaSuccess;
-  int device_ = 0, before_ = 0, sms_ = 0;
+  int before_ = 0, sms_ = 0;
   bool switched_ = false;
 };
 

@@ -37,7 +37,9 @@ namespace {
 using namespace octet;
 
 constexpr int kThreads = 256;
-static_assert(kThreads * 8 == kChunk, "a chunk is eight elements per thread");
+constexpr unsigned kChunk = kThreads * 8;         // AdamW: eight elements per thread
+constexpr int kNormOctets = 4;                    // the norm: four times that, all loaded before the first is used
+constexpr unsigned kNormChunk = kChunk * kNormOctets;
 static_assert(NB_OPTIM_BLOCK == 256, "a block is one warp's elements");
 
 // One tensor of the work list; its gradients' addresses follow the entries.
@@ -104,12 +106,29 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   return x ^ x >> 16;
 }
 
-// Rounds |z| <= 448 to e4m3 (as a float): down after u steps were added.
-__device__ __forceinline__ float round_random(float z, float u) {
-  int e = int(__float_as_uint(z) >> 23) - 130;  // log2 of the step between neighbours
-  e = e < -9 ? -9 : e;
-  const float step = __uint_as_float(uint32_t(e + 127) << 23), inv = __uint_as_float(uint32_t(127 - e) << 23);
-  return floorf(z * inv + u) * step;
+// Rounding |z| <= 448 (and an ulp) to e4m3 at random, to the code below
+// |z| / step + u steps with u = u16 / 65536. From 2^-6 on, a float whose low 20
+// mantissa bits are cut off is that code (the exponent's bias apart), and
+// adding u to those bits before the cut is the rounding. Below, neighbours are
+// 2^-9 apart, as they are from 2^-6 to 2^-5: 2^-6 is added, and its code
+// taken away again. `u24` is u16 << 8; the code plus 192 is in the top byte.
+__device__ __forceinline__ uint32_t round_random(float z, uint32_t u24) {
+  uint32_t b = __float_as_uint(z);
+  if (fabsf(z) < 0x1p-6f) b = __float_as_uint(fabsf(z) + 0x1p-6f) - (8u << 20);
+  return (b << 4) + u24;  // the sign is shifted out
+}
+
+// The codes of four such words.
+__device__ __forceinline__ uint32_t codes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t w = __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+  return ((w & 0x7f7f7f7fu) + 0x40404040u) ^ (w & 0x80808080u);  // 64 added to each byte
+}
+
+// The signs of four floats, where e4m3 has them.
+__device__ __forceinline__ uint32_t signs4(float a, float b, float c, float d) {
+  const uint32_t lo = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0073);
+  const uint32_t hi = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0073);
+  return __byte_perm(lo, hi, 0x5410) & 0x80808080u;
 }
 
 // Where a lane's eight elements are: neighbours, or 32 apart so that single
@@ -118,7 +137,7 @@ template <typename T>
 __device__ __forceinline__ void load8(const T* p, unsigned long long warp_base, int lane, long long left, bool vec,
                                       float (&f)[8]) {
   if (vec) {
-    unpack<T>(load<T, true>(p + warp_base + lane * 8, 8), f);
+    unpack<T>(load_oct(p + warp_base + lane * 8), f);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -130,7 +149,7 @@ template <typename T>
 __device__ __forceinline__ void store8(T* p, unsigned long long warp_base, int lane, long long left, bool vec,
                                        const float (&f)[8]) {
   if (vec) {
-    store<T, true>(p + warp_base + lane * 8, f, 8);
+    store_vec<T>(p + warp_base + lane * 8, pack<T>(f));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -155,10 +174,9 @@ __device__ __forceinline__ void load8_e4m3(const void* p, unsigned long long war
   from_e4m3(q, f);
 }
 
-__device__ __forceinline__ void store8_e4m3(void* p, unsigned long long warp_base, int lane, long long left, bool vec,
-                                            const float (&f)[8]) {
+__device__ __forceinline__ void store8_codes(void* p, unsigned long long warp_base, int lane, long long left, bool vec,
+                                             uint2 q) {
   uint8_t* b = static_cast<uint8_t*>(p) + warp_base;
-  const uint2 q = to_e4m3(f);
   if (vec) {
     *reinterpret_cast<uint2*>(b + lane * 8) = q;
   } else {
@@ -222,18 +240,30 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     }
     const float keep = 1.0f - lr * e.decay;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      g[j] *= scale;
+    for (int j = 0; j < 8; j += 2) {
+      const Pair gg = pair(g[j], g[j + 1]) * pair(scale, scale);
+      Pair mm = pair(m[j], m[j + 1]), vv = pair(v[j], v[j + 1]);
       if constexpr (S8) {
-        m[j] *= ms;
-        v[j] *= vs;
-        v[j] *= v[j];
+        mm = mm * pair(ms, ms);
+        vv = vv * pair(vs, vs);
+        vv = vv * vv;
       }
-      m[j] = m[j] * a.b1 + g[j] * a.b1c;
-      v[j] = v[j] * a.b2 + g[j] * g[j] * a.b2c;
-      const float r = sqrtf(v[j]);
-      p[j] = p[j] * keep - m[j] * size / (r * root + a.eps);
-      if constexpr (S8) v[j] = r;
+      mm = mm * pair(a.b1, a.b1) + gg * pair(a.b1c, a.b1c);
+      vv = vv * pair(a.b2, a.b2) + gg * gg * pair(a.b2c, a.b2c);
+      split(mm, m[j], m[j + 1]);
+      split(vv, v[j], v[j + 1]);
+      const float r0 = sqrtf(v[j]), r1 = sqrtf(v[j + 1]);
+      float n0, n1, d0, d1, k0, k1;
+      split(mm * pair(size, size), n0, n1);
+      split(pair(r0, r1) * pair(root, root) + pair(a.eps, a.eps), d0, d1);
+      split(pair(p[j], p[j + 1]) * pair(keep, keep), k0, k1);
+      // Off by two units in the last place at most, of a term far below p.
+      p[j] = k0 - __fdividef(n0, d0);
+      p[j + 1] = k1 - __fdividef(n1, d1);
+      if constexpr (S8) {
+        v[j] = r0;
+        v[j + 1] = r1;
+      }
     }
     store8<P>(static_cast<P*>(e.param), base, lane, left, vec, p);
     if constexpr (kCopy) store8<C>(static_cast<C*>(e.copy), base, lane, left, vec, p);
@@ -241,27 +271,27 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
       store8<float>(static_cast<float*>(e.m), base, lane, left, vec, m);
       store8<float>(static_cast<float*>(e.v), base, lane, left, vec, v);
     } else {
-      uint32_t mt = 0, vt = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        mt = max(mt, magnitude(m[j]));
-        vt = max(vt, magnitude(v[j]));
-      }
-      ms = scale_of(__reduce_max_sync(~0u, mt));
-      vs = scale_of(__reduce_max_sync(~0u, vt));
+      ms = scale_of(__reduce_max_sync(~0u, top_of(m)));
+      vs = scale_of(__reduce_max_sync(~0u, top_of(v)));
       const float mi = 1.0f / ms, vi = 1.0f / vs;
       const uint32_t key = a.seed + t * 0x165667B1u + e.index * 0x3C6EF35Fu + uint32_t(base >> 32) * 0x6A09E667u;
+      uint32_t at = (uint32_t(base) + (vec ? lane * 8 : lane)) * 0x9E3779B9u + key;
+      const uint32_t next = vec ? 0x9E3779B9u : 32u * 0x9E3779B9u;
+      uint32_t mw[8], vw[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t at = uint32_t(base) + (vec ? lane * 8 + j : j * 32 + lane);
-        const uint32_t bits = mix(at * 0x9E3779B9u + key);
-        const float z = fabsf(m[j]) * mi, y = v[j] * vi;
-        m[j] = copysignf(round_random(z > kE4m3Max ? kE4m3Max : z, float(bits >> 16) * 0x1p-16f), m[j]);
-        const float q = round_random(y > kE4m3Max ? kE4m3Max : y, float(bits & 0xffffu) * 0x1p-16f);
-        v[j] = v[j] > 0.0f && q < 0x1p-9f ? 0x1p-9f : q;
+        const uint32_t bits = mix(at);
+        at += next;
+        mw[j] = round_random(m[j] * mi, __byte_perm(bits, 0, 0x4324));  // the upper half
+        // A positive root has the least code at least, which is 2^-9.
+        const float y = v[j] * vi;
+        vw[j] = round_random(v[j] > 0.0f ? fmaxf(y, 0x1p-9f) : y, __byte_perm(bits, 0, 0x4104));  // the lower half
       }
-      store8_e4m3(e.m, base, lane, left, vec, m);
-      store8_e4m3(e.v, base, lane, left, vec, v);
+      store8_codes(e.m, base, lane, left, vec,
+                   make_uint2(codes4(mw[0], mw[1], mw[2], mw[3]) | signs4(m[0], m[1], m[2], m[3]),
+                              codes4(mw[4], mw[5], mw[6], mw[7]) | signs4(m[4], m[5], m[6], m[7])));
+      store8_codes(e.v, base, lane, left, vec,
+                   make_uint2(codes4(vw[0], vw[1], vw[2], vw[3]), codes4(vw[4], vw[5], vw[6], vw[7])));
       if (lane == 0) {
         e.m_scale[base >> 8] = ms;
         e.v_scale[base >> 8] = vs;
@@ -290,22 +320,59 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
   for (unsigned c = blockIdx.x; c < a.chunks; c += gridDim.x) {
     while (i + 1 < a.count && entries[i + 1].first <= c) ++i;
     const GradEntry& e = entries[i];
-    const unsigned long long base = (unsigned long long)(c - e.first) * kChunk + (unsigned)warp * 256u;
+    const unsigned long long base =
+        (unsigned long long)(c - e.first) * kNormChunk + (unsigned)warp * (256u * kNormOctets);
     if (base >= e.size) continue;
     const long long left = (long long)(e.size - base);
-    const bool vec = e.vec && left >= 256;
-    float g[8], s = 0.0f;
-    load8<G>(reinterpret_cast<const G*>(grads[(size_t)i * a.parts]), base, lane, left, vec, g);
+    const unsigned long long* from = grads + (size_t)i * a.parts;
+    if (e.vec && left >= 256 * kNormOctets) {
+      Oct<G> o[kNormOctets];
+      float g[kNormOctets][8];
+      const G* p = reinterpret_cast<const G*>(from[0]) + base + lane * 8;
+#pragma unroll
+      for (int u = 0; u < kNormOctets; ++u) o[u] = load_oct(p + u * 256);
+#pragma unroll
+      for (int u = 0; u < kNormOctets; ++u) unpack<G>(o[u], g[u]);
 #pragma unroll 1
-    for (int k = 1; k < a.parts; ++k) {
-      float f[8];
-      load8<G>(reinterpret_cast<const G*>(grads[(size_t)i * a.parts + k]), base, lane, left, vec, f);
+      for (int k = 1; k < a.parts; ++k) {
+        p = reinterpret_cast<const G*>(from[k]) + base + lane * 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] += f[j];
+        for (int u = 0; u < kNormOctets; ++u) o[u] = load_oct(p + u * 256);
+#pragma unroll
+        for (int u = 0; u < kNormOctets; ++u) {
+          float f[8];
+          unpack<G>(o[u], f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[u][j] += f[j];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kNormOctets; ++u) {
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(g[u][j], g[u][j], s);
+        total += double(s);
+      }
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < kNormOctets && u * 256 < left; ++u) {
+        float g[8], s = 0.0f;
+        const unsigned long long at = base + u * 256;
+        const long long rest = left - u * 256;
+        const bool vec = e.vec && rest >= 256;
+        load8<G>(reinterpret_cast<const G*>(from[0]), at, lane, rest, vec, g);
+#pragma unroll 1
+        for (int k = 1; k < a.parts; ++k) {
+          float f[8];
+          load8<G>(reinterpret_cast<const G*>(from[k]), at, lane, rest, vec, f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[j] += f[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(g[j], g[j], s);
+        total += double(s);
+      }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(g[j], g[j], s);
-    total += double(s);
   }
   total = warp_sum(total);
   if (lane == 0) sums[warp] = total;
@@ -410,10 +477,10 @@ struct NormHandle {
 
 template <typename E, typename Fill>
 std::vector<Launch> build_launches(const uint64_t* sizes, int count, int parts, const void* const* grad, int sms,
-                                   Fill fill) {
+                                   unsigned chunk, Fill fill) {
   constexpr int kWords = sizeof(E) / 8;
   std::vector<Launch> out;
-  for (const TableLaunch& t : pack_tensors(sizes, size_t(count), kLargeWords / (kWords + parts))) {
+  for (const TableLaunch& t : pack_tensors(sizes, size_t(count), kLargeWords / (kWords + parts), chunk)) {
     Launch l;
     l.count = int(t.tensor.size());
     l.chunks = t.chunks;
@@ -480,8 +547,8 @@ extern "C" void* nb_adamw_create(const nb_adamw_t* a, char* err, size_t errcap) 
   if (!s8 && a->state_dtype != NB_OPTIM_FLOAT32)
     return refuse("bad arguments: states are ncclFloat32 or ncclFloat8e4m3");
   if (s8 && (!a->m_scale || !a->v_scale)) return refuse("bad arguments: 8-bit states need their scales");
-  if (!(a->beta1 >= 0 && a->beta1 < 1) || !(a->beta2 >= 0 && a->beta2 < 1) || !(a->eps > 0) || !std::isfinite(a->eps))
-    return refuse("bad arguments: 0 <= beta < 1 and eps > 0");
+  if (!(a->beta1 >= 0 && a->beta1 < 1) || !(a->beta2 >= 0 && a->beta2 < 1) || !(a->eps >= 1.2e-38) || !(a->eps <= 3.4e38))
+    return refuse("bad arguments: 0 <= beta < 1 and eps a positive normal fp32 number");
   if (const char* why = check_list(a->size, a->count, a->parts, a->grad, gs)) return refuse(why);
   for (int i = 0; i < a->count; ++i) {
     if (!std::isfinite(a->weight_decay[i])) return refuse("bad arguments: weight_decay must be finite");
@@ -504,7 +571,7 @@ extern "C" void* nb_adamw_create(const nb_adamw_t* a, char* err, size_t errcap) 
     h->seed = a->seed * 0x27D4EB2Fu;
     h->kernel[0] = adamw_for<kSmallWords>(a->param_dtype, a->copy_dtype, a->grad_dtype, s8);
     h->kernel[1] = adamw_for<kLargeWords>(a->param_dtype, a->copy_dtype, a->grad_dtype, s8);
-    h->launches = build_launches<Entry>(a->size, a->count, a->parts, a->grad, dev.sms(), [&](int i, Entry& e) {
+    h->launches = build_launches<Entry>(a->size, a->count, a->parts, a->grad, dev.sms(), kChunk, [&](int i, Entry& e) {
       e.param = a->param[i];
       e.copy = cs ? a->copy[i] : nullptr;
       e.m = a->m[i];
@@ -604,7 +671,7 @@ extern "C" void* nb_grad_norm_create(int device, int count, int parts, int dtype
     h->parts = parts;
     h->kernel[0] = grad_norm_for<kSmallWords>(dtype);
     h->kernel[1] = grad_norm_for<kLargeWords>(dtype);
-    h->launches = build_launches<GradEntry>(size, count, parts, grad, dev.sms(), [&](int i, GradEntry& e) {
+    h->launches = build_launches<GradEntry>(size, count, parts, grad, dev.sms(), kNormChunk, [&](int i, GradEntry& e) {
       bool vec = true;
       for (int p = 0; p < parts; ++p)
         vec = vec && on_boundary(grad[size_t(i) * size_t(parts) + size_t(p)], size_t(gs) * 8);

@@ -27,10 +27,19 @@ namespace {
 using namespace octet;
 
 constexpr int kLongThreads = 1024;
+constexpr int kRingThreads = 512;
+// Threads of a norm's block at most: 64 registers do for one aligned sum and its residual.
+__host__ __device__ constexpr int max_threads(bool vec, bool many) { return vec && !many ? 1024 : 512; }
 
 struct Rows {
   const void* p;
   long long outer, inner;
+};
+
+// r / inner and r % inner for row numbers below 2^31 by a multiplication
+// (Granlund and Montgomery, 1994): q = (mulhi(r, magic) + r) >> shift.
+struct RowSplit {
+  unsigned inner, magic, shift;
 };
 
 struct FwdArgs {
@@ -41,9 +50,10 @@ struct FwdArgs {
   float* scale;
   void* h;
   float* rstd;
-  long long rows, inner;
-  int hidden, parts, wf32, group, tpr, groups;
-  float eps;
+  long long rows;
+  RowSplit split;
+  int hidden, parts, group, tpr, groups;
+  float eps, inv_hidden;
 };
 
 struct BwdArgs {
@@ -52,23 +62,26 @@ struct BwdArgs {
   const float* rstd;
   void* dx;
   float* partial;  // [blocks][hidden]
-  long long rows, inner;
-  int hidden, wf32, tpr;
+  long long rows;
+  RowSplit split;
+  int hidden, tpr;
+  float inv_hidden;
 };
 
-template <typename T>
-__device__ __forceinline__ const T* row_of(const Rows& r, long long row, long long inner) {
-  // One row dimension is the usual case and needs no division.
-  if (inner == 1) return static_cast<const T*>(r.p) + row * r.outer;
-  const long long o = row / inner;
-  return static_cast<const T*>(r.p) + o * r.outer + (row - o * inner) * r.inner;
-}
+// A row's place in every tensor of a call.
+struct Row {
+  long long outer, inner;
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_weight(const void* w, int wf32, int col, int left, float (&f)[8]) {
-  if (wf32) unpack<float>(load<float, VEC>(static_cast<const float*>(w) + col, left), f);
-  else unpack<T>(load<T, VEC>(static_cast<const T*>(w) + col, left), f);
-}
+  __device__ __forceinline__ Row(long long r, const RowSplit& s) {
+    const unsigned n = unsigned(r), q = (__umulhi(n, s.magic) + n) >> s.shift;
+    outer = q;
+    inner = n - q * s.inner;
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* of(const Rows& t) const {
+    return static_cast<const T*>(t.p) + outer * t.outer + inner * t.inner;
+  }
+};
 
 // Sum over the threads of one row: `tpr` lanes of a warp (a power of two), or
 // the whole block (tpr > 32), whose warps meet in `red`.
@@ -95,323 +108,585 @@ __device__ __forceinline__ uint32_t row_max(uint32_t m, int tpr, uint32_t* red) 
   return __reduce_max_sync(~0u, lane < warps ? red[lane] : 0u);
 }
 
-// The sum of every partial and the residual at one octet.
-template <typename T, bool VEC>
-__device__ __forceinline__ void sum_octet(const FwdArgs& a, long long row, int col, int left, float (&h)[8]) {
-  unpack<T>(load<T, VEC>(row_of<T>(a.x[0], row, a.inner) + col, left), h);
-#pragma unroll 1
-  for (int s = 1; s < a.parts; ++s) {
-    float f[8];
-    unpack<T>(load<T, VEC>(row_of<T>(a.x[s], row, a.inner) + col, left), f);
+// A thread's K times eight elements of a row: where the first of each eight
+// is, how far apart they are, and how much of the row is left from there on.
+// The k-th eight of a warp's 32 threads (of a row's `tpr`, if fewer) are 256
+// (8 tpr) neighbours; each thread has eight of them in a row (VEC), or every
+// 32nd (tpr-th). Without any (left <= 0) it reads the row's first ones and
+// drops them.
+template <int K, bool VEC>
+struct Part {
+  int lane, step, at[K], left[K];
+
+  __device__ __forceinline__ Part(int lane_, int tpr, int hidden) : lane(lane_) {
+    const int width = tpr < 32 ? tpr : 32, in = lane & (width - 1);
+    step = VEC ? 1 : width;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] += f[j];
+    for (int k = 0; k < K; ++k) {
+      at[k] = (lane - in + k * tpr) * 8 + (VEC ? in * 8 : in);
+      left[k] = hidden - at[k];
+      if (left[k] <= 0) at[k] = 0;
+    }
   }
-  if (a.residual.p) {
-    float f[8];
-    unpack<T>(load<T, VEC>(row_of<T>(a.residual, row, a.inner) + col, left), f);
+};
+
+// A thread's elements of one row of a tensor.
+template <typename T, bool VEC, int K>
+struct Load {
+  Raw<T, VEC> raw[K];
+
+  __device__ __forceinline__ void load(const T* row, const Part<K, VEC>& part) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] += f[j];
+    for (int k = 0; k < K; ++k) raw[k].load(row + part.at[k], part.step, part.left[k]);
   }
+  __device__ __forceinline__ void get(int k, Pair (&f)[4]) const { raw[k].get(f); }
+};
+
+__device__ __forceinline__ void add(Pair (&h)[4], const Pair (&f)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = h[j] + f[j];
 }
 
+__device__ __forceinline__ float sum_of(Pair p) {
+  float a, b;
+  split(p, a, b);
+  return a + b;
+}
+
+// Eight values times their scales' reciprocals to e4m3.
 template <bool VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[8], float inv, int left) {
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[8], const float (&inv)[8], int step, int left) {
   float z[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) z[j] = f[j] * inv;
+  for (int j = 0; j < 8; j += 2) split(pair(f[j], f[j + 1]) * pair(inv[j], inv[j + 1]), z[j], z[j + 1]);
   const uint2 q = to_e4m3(z);
   if constexpr (VEC) {
-    *reinterpret_cast<uint2*>(p) = q;
+    if (left > 0) *reinterpret_cast<uint2*>(p) = q;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < left) p[j] = uint8_t((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+      if (j * step < left) p[j * step] = uint8_t((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
   }
 }
 
-// The scale of each group of 32, 64 or 128 columns (neighbouring octets are
-// held by neighbouring lanes), stored by the group's first lane.
-__device__ __forceinline__ float group_scale(const FwdArgs& a, uint32_t top, int tpr, long long row, int col,
-                                             bool here) {
-  int lanes = a.group >> 3;
-  if (lanes > tpr) lanes = tpr;  // the row is shorter than the group
-  for (int o = lanes >> 1; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
-  const float s = scale_of(top);
-  if (here && (col % a.group) == 0) a.scale[row * a.groups + col / a.group] = s;
-  return s;
+// 1 / scale, for a scale of at least 2^-126: off by an ulp at most, so that a
+// value within that of the middle between two codes may take either.
+__device__ __forceinline__ float reciprocal(float scale) { return __fdividef(1.0f, scale); }
+
+// The reciprocals of the scales of groups of 32, 64 or 128 columns, one for each
+// of a thread's eight values; the group's first thread stores its scale. `whole`: the
+// largest magnitude of the row's part, where a group is wider than that.
+template <bool VEC>
+__device__ __forceinline__ void group_scales(const FwdArgs& a, const float (&y)[8], uint32_t whole, int tpr,
+                                             long long row, int at, int left, float (&inv)[8]) {
+  const int width = tpr < 32 ? tpr : 32;
+  float* to = a.scale + row * a.groups;
+  if constexpr (VEC) {  // a thread's values are in one group, with its neighbours
+    uint32_t top = left > 0 ? top_of(y) : 0;
+    int lanes = a.group >> 3;
+    if (lanes > width) {
+      lanes = width;
+      top = whole;
+    }
+    for (int o = lanes >> 1; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+    const float s = scale_of(top), i = reciprocal(s);
+    if (left > 0 && (at & (a.group - 1)) == 0) to[unsigned(at) / unsigned(a.group)] = s;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) inv[j] = i;
+  } else {  // a group is `per` neighbouring j of all the row's lanes
+    const int per = a.group / width;
+    uint32_t top[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top[j] = j * width < left ? magnitude(y[j]) : 0;
+    if (per > 8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top[j] = whole;
+    }
+#pragma unroll
+    for (int half = 1; half < 8; half *= 2)
+      if (per > half) {
+        uint32_t other[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) other[j] = top[j ^ half];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top[j] = max(top[j], other[j]);
+      }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      for (int o = width >> 1; o; o >>= 1) top[j] = max(top[j], __shfl_xor_sync(~0u, top[j], o));
+      const float s = scale_of(top[j]);
+      inv[j] = reciprocal(s);
+      const int col = at + j * width;
+      if (j * width < left && (col & (a.group - 1)) == 0) to[unsigned(col) / unsigned(a.group)] = s;
+    }
+  }
 }
 
-// K octets per thread, the row in registers. Octet k of thread t is t + k * tpr.
-template <typename T, bool F8, bool VEC, int K>
-__global__ void __launch_bounds__(K <= 2 ? 1024 : 512) norm_kernel(const __grid_constant__ FwdArgs a) {
+// One row per tpr threads, in registers: every load is issued before the
+// first value is used, and a row's threads meet once (twice with one e4m3
+// scale per row). W: the weight's type; MANY: more than one partial sum.
+template <typename T, typename W, bool F8, bool VEC, bool MANY, int K>
+__global__ void __launch_bounds__(max_threads(VEC, MANY)) norm_kernel(const __grid_constant__ FwdArgs a) {
   __shared__ float red[32];
   __shared__ uint32_t top_red[32];
-  const int tpr = a.tpr;
+  const int tpr = a.tpr, hidden = a.hidden;
   const int lane = tpr > 32 ? threadIdx.x : threadIdx.x & (tpr - 1);
   const long long row = tpr > 32 ? (long long)blockIdx.x
                                  : (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
   const bool live = row < a.rows;  // every thread stays for the shuffles
-  float h[K][8], s = 0.0f;
+  const Row from(live ? row : 0, a.split);
+  Part<K, VEC> part(lane, tpr, hidden);
+  // Four partial sums at a time, with the first of them the residual too.
+  constexpr int N = MANY ? 4 : 1;
+  Load<T, VEC, K> xv[N], rv;
+  Load<W, VEC, K> wv;
+  Pair h[K][4], f[4];
+#pragma unroll 1
+  for (int s0 = 0; s0 < (MANY ? a.parts : 1); s0 += N) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int col = (lane + k * tpr) * 8, left = live ? a.hidden - col : 0;
-    if (left > 0) {
-      sum_octet<T, VEC>(a, row, col, left, h[k]);
-    } else {
+    for (int i = 0; i < N; ++i)
+      if (s0 + i < a.parts) xv[i].load(from.of<T>(a.x[s0 + i]), part);
+    if (s0 == 0 && a.residual.p) rv.load(from.of<T>(a.residual), part);
+    if (s0 == 0) wv.load(static_cast<const W*>(a.weight), part);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[k][j] = 0.0f;
+    for (int k = 0; k < K; ++k) {
+      if (s0 == 0) {
+        xv[0].get(k, h[k]);
+      } else {
+        xv[0].get(k, f);
+        add(h[k], f);
+      }
+#pragma unroll
+      for (int i = 1; i < N; ++i)
+        if (s0 + i < a.parts) {
+          xv[i].get(k, f);
+          add(h[k], f);
+        }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(h[k][j], h[k][j], s);
   }
-  float w[K][8];
+  if (a.residual.p) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int col = (lane + k * tpr) * 8, left = live ? a.hidden - col : 0;
-    if (left > 0) load_weight<T, VEC>(a.weight, a.wf32, col, left, w[k]);
-    else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[k][j] = 0.0f;
+    for (int k = 0; k < K; ++k) {
+      rv.get(k, f);
+      add(h[k], f);
     }
   }
+  if (!live) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) part.left[k] = 0;
+  }
+  Pair sum = pair(0.0f, 0.0f);
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (part.left[k] > 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = fma(h[k][j], h[k][j], sum);
+    }
+  const long long out = row * a.hidden;
   if (a.h) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * tpr) * 8, left = live ? a.hidden - col : 0;
-      if (left > 0) store<T, VEC>(static_cast<T*>(a.h) + row * a.hidden + col, h[k], left);
+      float e[8];
+      split(h[k], e);
+      store8<T, VEC>(static_cast<T*>(a.h) + out + part.at[k], e, part.step, part.left[k]);
     }
   }
-  s = row_sum(s, tpr, red);
-  const float rstd = 1.0f / sqrtf(s / float(a.hidden) + a.eps);
+  const float s = row_sum(sum_of(sum), tpr, red);
+  const float rstd = rsqrtf(fmaf(s, a.inv_hidden, a.eps));
   if (live && lane == 0) a.rstd[row] = rstd;
-  uint32_t top = 0;
+  const Pair r2 = pair(rstd, rstd);
+  float y[K][8];
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int k = 0; k < K; ++k) {
+    wv.get(k, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      h[k][j] = h[k][j] * rstd * w[k][j];
-      if constexpr (F8) top = max(top, magnitude(h[k][j]));
-    }
+    for (int j = 0; j < 4; ++j) f[j] = h[k][j] * r2 * f[j];
+    split(f, y[k]);
+  }
   if constexpr (!F8) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * tpr) * 8, left = live ? a.hidden - col : 0;
-      if (left > 0) store<T, VEC>(static_cast<T*>(a.y) + row * a.hidden + col, h[k], left);
-    }
+    for (int k = 0; k < K; ++k)
+      store8<T, VEC>(static_cast<T*>(a.y) + out + part.at[k], y[k], part.step, part.left[k]);
   } else {
-    float inv = 0.0f;
+    uint32_t most = 0;
+    if (a.group == 0 || a.group > 8 * tpr) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (part.left[k] > 0) most = max(most, top_of<VEC>(y[k], part.step, part.left[k]));
+    }
+    float inv[8];
     if (a.group == 0) {
-      const float scale = scale_of(row_max(top, tpr, top_red));
+      const float scale = scale_of(row_max(most, tpr, top_red));
       if (live && lane == 0) a.scale[row] = scale;
-      inv = 1.0f / scale;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) inv[j] = reciprocal(scale);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * tpr) * 8, left = live ? a.hidden - col : 0;
-      if (a.group) {
-        top = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude(h[k][j]));
-        inv = 1.0f / group_scale(a, top, tpr, row, col, left > 0);
-      }
-      if (left > 0) store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + row * a.hidden + col, h[k], inv, left);
+      if (a.group) group_scales<VEC>(a, y[k], most, tpr, row, part.at[k], part.left[k], inv);
+      store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + out + part.at[k], y[k], inv, part.step, part.left[k]);
     }
+  }
+}
+
+// The sum of every partial and the residual at eight elements.
+template <typename T, bool VEC>
+__device__ __forceinline__ void sum8(const FwdArgs& a, const Row& from, const Part<1, VEC>& part, Pair (&h)[4]) {
+  Load<T, VEC, 1> v;
+  Pair f[4];
+  v.load(from.of<T>(a.x[0]), part);
+  v.get(0, h);
+#pragma unroll 1
+  for (int s = 1; s < a.parts + (a.residual.p ? 1 : 0); ++s) {
+    v.load(from.of<T>(s < a.parts ? a.x[s] : a.residual), part);
+    v.get(0, f);
+    add(h, f);
+  }
+}
+
+// The turns that a block of kLongThreads takes over a long row: turn k is the
+// k-th eight elements of its threads. Whole warps take every turn.
+template <bool VEC, typename F>
+__device__ __forceinline__ void each_turn(int hidden, F f) {
+  const int turns = (hidden + 8 * kLongThreads - 1) / (8 * kLongThreads);
+  Part<1, VEC> part(threadIdx.x, kLongThreads, hidden);
+  const int first = part.at[0];  // 0 too for a thread without elements in a row below one turn
+  for (int k = 0; k < turns; ++k) {
+    part.at[0] = first + k * 8 * kLongThreads;
+    part.left[0] = hidden - part.at[0];
+    if (part.left[0] <= 0) part.at[0] = 0;
+    f(part);
   }
 }
 
 // Rows that do not fit the registers of a block: the sum is formed again in
 // each pass over the row (from L2), and h is written in the last one, so that
 // it may still replace an input.
-template <typename T, bool F8, bool VEC>
+template <typename T, typename W, bool F8, bool VEC>
 __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_constant__ FwdArgs a) {
   __shared__ float red[32];
   __shared__ uint32_t top_red[32];
-  const long long row = blockIdx.x;
-  // Whole warps take every turn, for the shuffles of a group's scale.
-  const int turns = (a.hidden + 8 * kLongThreads - 1) / (8 * kLongThreads);
-  float s = 0.0f;
-  for (int k = 0; k < turns; ++k) {
-    const int col = (k * kLongThreads + threadIdx.x) * 8, left = a.hidden - col;
-    if (left <= 0) continue;
-    float h[8];
-    sum_octet<T, VEC>(a, row, col, left, h);
+  const long long row = blockIdx.x, out = row * a.hidden;
+  const Row from(row, a.split);
+  const auto normal = [&](const Part<1, VEC>& part, float rstd, const Pair (&h)[4], float (&y)[8]) {
+    Load<W, VEC, 1> wv;
+    Pair w[4];
+    wv.load(static_cast<const W*>(a.weight), part);
+    wv.get(0, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(h[j], h[j], s);
-  }
-  s = row_sum(s, kLongThreads, red);
-  const float rstd = 1.0f / sqrtf(s / float(a.hidden) + a.eps);
+    for (int j = 0; j < 4; ++j) w[j] = h[j] * pair(rstd, rstd) * w[j];
+    split(w, y);
+  };
+  Pair sum = pair(0.0f, 0.0f);
+  each_turn<VEC>(a.hidden, [&](const Part<1, VEC>& part) {
+    if (part.left[0] <= 0) return;
+    Pair h[4];
+    sum8<T, VEC>(a, from, part, h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = fma(h[j], h[j], sum);
+  });
+  const float s = row_sum(sum_of(sum), kLongThreads, red);
+  const float rstd = rsqrtf(fmaf(s, a.inv_hidden, a.eps));
   if (threadIdx.x == 0) a.rstd[row] = rstd;
-  float inv = 0.0f;
+  float inv[8] = {};
   if (F8 && a.group == 0) {
     uint32_t top = 0;
-    for (int k = 0; k < turns; ++k) {
-      const int col = (k * kLongThreads + threadIdx.x) * 8, left = a.hidden - col;
-      if (left <= 0) continue;
-      float h[8], w[8];
-      sum_octet<T, VEC>(a, row, col, left, h);
-      load_weight<T, VEC>(a.weight, a.wf32, col, left, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, magnitude(h[j] * rstd * w[j]));
-    }
+    each_turn<VEC>(a.hidden, [&](const Part<1, VEC>& part) {
+      if (part.left[0] <= 0) return;
+      Pair h[4];
+      float y[8];
+      sum8<T, VEC>(a, from, part, h);
+      normal(part, rstd, h, y);
+      top = max(top, top_of<VEC>(y, part.step, part.left[0]));
+    });
     const float scale = scale_of(row_max(top, kLongThreads, top_red));
     if (threadIdx.x == 0) a.scale[row] = scale;
-    inv = 1.0f / scale;
-  }
-  for (int k = 0; k < turns; ++k) {
-    const int col = (k * kLongThreads + threadIdx.x) * 8, left = a.hidden - col;
-    float h[8] = {}, w[8];
-    if (left > 0) {
-      sum_octet<T, VEC>(a, row, col, left, h);
-      if (a.h) store<T, VEC>(static_cast<T*>(a.h) + row * a.hidden + col, h, left);
-      load_weight<T, VEC>(a.weight, a.wf32, col, left, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = h[j] * rstd * w[j];
+    for (int j = 0; j < 8; ++j) inv[j] = reciprocal(scale);
+  }
+  each_turn<VEC>(a.hidden, [&](const Part<1, VEC>& part) {
+    const int at = part.at[0], left = part.left[0];
+    Pair h[4] = {};
+    float y[8] = {}, e[8];
+    if (left > 0) {
+      sum8<T, VEC>(a, from, part, h);
+      normal(part, rstd, h, y);
+      split(h, e);
+      if (a.h) store8<T, VEC>(static_cast<T*>(a.h) + out + at, e, part.step, left);
     }
     if constexpr (F8) {
-      if (a.group) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude(h[j]));
-        inv = 1.0f / group_scale(a, top, kLongThreads, row, col, left > 0);
-      }
-      if (left > 0) store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + row * a.hidden + col, h, inv, left);
+      if (a.group) group_scales<VEC>(a, y, 0, kLongThreads, row, at, left, inv);
+      store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + out + at, y, inv, part.step, left);
     } else {
-      if (left > 0) store<T, VEC>(static_cast<T*>(a.y) + row * a.hidden + col, h, left);
+      store8<T, VEC>(static_cast<T*>(a.y) + out + at, y, part.step, left);
+    }
+  });
+}
+
+// A row of the gradient, from this thread's elements: adds to dw's part and
+// stores dx.
+template <typename T, typename W, bool VEC, int K, typename In>
+__device__ __forceinline__ void finish_grad(const BwdArgs& a, long long row, bool live, const Part<K, VEC>& part,
+                                            const In& dy, const In& h, const In& dh, float rstd,
+                                            const Load<W, VEC, K>& wv, Pair (&acc)[K][4], float* red) {
+  Pair g[K][4], n[K][4], sum = pair(0.0f, 0.0f);
+  const Pair r2 = pair(rstd, rstd);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    Pair w[4];
+    dy.get(k, g[k]);
+    h.get(k, n[k]);
+    wv.get(k, w);
+    if (part.left[k] > 0 && live) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        n[k][j] = n[k][j] * r2;
+        acc[k][j] = fma(g[k][j], n[k][j], acc[k][j]);
+        g[k][j] = g[k][j] * w[j];
+        sum = fma(g[k][j], n[k][j], sum);
+      }
+    }
+  }
+  const float c = row_sum(sum_of(sum), a.tpr, red) * -a.inv_hidden;
+  const Pair c2 = pair(c, c);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    Pair e[4];
+    if (a.dh.p) dh.get(k, e);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Pair t = fma(n[k][j], c2, g[k][j]);
+      e[j] = a.dh.p ? fma(t, r2, e[j]) : t * r2;
+    }
+    float f[8];
+    split(e, f);
+    store8<T, VEC>(static_cast<T*>(a.dx) + row * a.hidden + part.at[k], f, part.step, live ? part.left[k] : 0);
+  }
+}
+
+// The block's part of dw: its rows are fixed, and with several rows at once
+// its slots are added in order.
+template <int K, bool VEC>
+__device__ __forceinline__ void store_partial(const BwdArgs& a, const Part<K, VEC>& part, const Pair (&acc)[K][4],
+                                              float* slots) {
+  const int tpr = a.tpr;
+  float* to = a.partial + (long long)blockIdx.x * a.hidden;
+  if (tpr <= 32) to = slots + (threadIdx.x / tpr) * a.hidden;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float f[8];
+    split(acc[k], f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j * part.step < part.left[k]) to[part.at[k] + j * part.step] = f[j];
+  }
+  if (tpr <= 32) {
+    __syncthreads();
+    const int per = blockDim.x / tpr;
+    for (int col = threadIdx.x; col < a.hidden; col += blockDim.x) {
+      float s = 0.0f;
+      for (int q = 0; q < per; ++q) s += slots[q * a.hidden + col];
+      a.partial[(long long)blockIdx.x * a.hidden + col] = s;
     }
   }
 }
 
-// Each block walks over rows and keeps its columns' part of dw in registers
-// (fixed rows per block, so the sum's order is fixed); the parts go to
-// `partial` and dw_kernel adds them in block order.
-template <typename T, bool VEC, int K>
-__global__ void __launch_bounds__(1024) norm_backward_kernel(const __grid_constant__ BwdArgs a) {
+template <int K>
+__device__ __forceinline__ void clear(Pair (&acc)[K][4]) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[k][j] = pair(0.0f, 0.0f);
+}
+
+// Each block walks over rows and keeps its columns' part of dw in registers;
+// the parts go to `partial` and dw_kernel adds them in block order.
+template <typename T, typename W, bool VEC, int K>
+__global__ void __launch_bounds__(kRingThreads) norm_backward_kernel(const __grid_constant__ BwdArgs a) {
   __shared__ float red[2][32];
-  __shared__ float slots[256 * 8];
+  __shared__ float slots[256 * 8 * K];
   const int tpr = a.tpr;
   const int lane = tpr > 32 ? threadIdx.x : threadIdx.x & (tpr - 1);
   const int per = tpr > 32 ? 1 : blockDim.x / tpr, slot = tpr > 32 ? 0 : threadIdx.x / tpr;
-  float acc[K][8], w[K][8];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int col = (lane + k * tpr) * 8, left = a.hidden - col;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[k][j] = w[k][j] = 0.0f;
-    if (left > 0) load_weight<T, VEC>(a.weight, a.wf32, col, left, w[k]);
-  }
+  const Part<K, VEC> part(lane, tpr, a.hidden);
+  Pair acc[K][4];
+  Load<W, VEC, K> wv;
+  wv.load(static_cast<const W*>(a.weight), part);
+  clear<K>(acc);
+  const long long stride = (long long)gridDim.x * per;
   int turn = 0;
-  for (long long base = (long long)blockIdx.x * per; base < a.rows; base += (long long)gridDim.x * per) {
-    const long long row = base + slot;
+  for (long long row = (long long)blockIdx.x * per + slot; row - slot < a.rows; row += stride, ++turn) {
     const bool live = row < a.rows;
-    Oct<T> dy[K], h[K], dh[K];
+    const long long r = live ? row : a.rows - 1;
+    const Row from(r, a.split);
+    Load<T, VEC, K> dy, h, dh;
+    dy.load(from.of<T>(a.dy), part);
+    h.load(from.of<T>(a.h), part);
+    if (a.dh.p) dh.load(from.of<T>(a.dh), part);
+    finish_grad<T, W, VEC, K>(a, row, live, part, dy, h, dh, a.rstd[r], wv, acc, red[turn & 1]);
+  }
+  store_partial<K, VEC>(a, part, acc, slots);
+}
+
+// A thread's own ring in shared memory: kStages rows of its octets of a 16-bit
+// type, brought by 16-byte asynchronous copies. Only the thread itself reads
+// them, so a stage needs no barrier: the thread waits for its own copies.
+// Copies of later rows are in flight while a row is reduced, without a
+// register held for them.
+constexpr int kStages = 4;
+
+template <typename T, int K>
+struct Ring {
+  uint4* base;
+  int sources;
+
+  __device__ __forceinline__ uint4* slot(int stage, int source, int k) const {
+    return base + ((stage * sources + source) * K + k) * int(blockDim.x) + threadIdx.x;
+  }
+  __device__ __forceinline__ void fetch(int stage, int source, const T* row, const Part<K, true>& part) const {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * tpr) * 8, left = live ? a.hidden - col : 0;
-      dy[k] = h[k] = dh[k] = Oct<T>{};
-      if (left > 0) {
-        dy[k] = load<T, VEC>(row_of<T>(a.dy, row, a.inner) + col, left);
-        h[k] = load<T, VEC>(row_of<T>(a.h, row, a.inner) + col, left);
-        if (a.dh.p) dh[k] = load<T, VEC>(row_of<T>(a.dh, row, a.inner) + col, left);
-      }
+    for (int k = 0; k < K; ++k)
+      if (part.left[k] > 0)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         uint32_t(__cvta_generic_to_shared(slot(stage, source, k)))),
+                     "l"(row + part.at[k])
+                     : "memory");
+  }
+  __device__ __forceinline__ void read(int stage, int source, Load<T, true, K>& o) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) o.raw[k].o.v[0] = *slot(stage, source, k);
+  }
+};
+
+// The same with the next rows on their way (octets on their boundary). A
+// thread without an octet or a row reads what the ring happens to hold and
+// drops it.
+template <typename T, typename W, int K>
+__global__ void __launch_bounds__(kRingThreads) norm_backward_ring_kernel(const __grid_constant__ BwdArgs a) {
+  extern __shared__ uint4 smem[];
+  __shared__ float red[2][32];
+  const int tpr = a.tpr;
+  const int lane = tpr > 32 ? threadIdx.x : threadIdx.x & (tpr - 1);
+  const int per = tpr > 32 ? 1 : blockDim.x / tpr, slot = tpr > 32 ? 0 : threadIdx.x / tpr;
+  const Part<K, true> part(lane, tpr, a.hidden);
+  const Ring<T, K> ring{smem, a.dh.p ? 3 : 2};
+  const long long stride = (long long)gridDim.x * per;
+  long long ahead = (long long)blockIdx.x * per + slot;
+  float rstds[kStages];  // of the rows on their way
+  const auto fetch = [&](int stage, float& rstd) {
+    rstd = 0.0f;
+    if (ahead < a.rows) {
+      const Row from(ahead, a.split);
+      ring.fetch(stage, 0, from.of<T>(a.dy), part);
+      ring.fetch(stage, 1, from.of<T>(a.h), part);
+      if (a.dh.p) ring.fetch(stage, 2, from.of<T>(a.dh), part);
+      rstd = a.rstd[ahead];
     }
-    const float rstd = live ? a.rstd[row] : 0.0f;
-    float c = 0.0f;
+    ahead += stride;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float d[8], n[8];
-      unpack<T>(dy[k], d);
-      unpack<T>(h[k], n);
+  for (int s = 0; s < kStages - 1; ++s) fetch(s, rstds[s]);
+  Pair acc[K][4];
+  Load<W, true, K> wv;
+  wv.load(static_cast<const W*>(a.weight), part);
+  clear<K>(acc);
+  for (long long row = (long long)blockIdx.x * per + slot; row - slot < a.rows;) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        n[j] *= rstd;
-        acc[k][j] = fmaf(d[j], n[j], acc[k][j]);
-        c = fmaf(d[j] * w[k][j], n[j], c);
-      }
-    }
-    c = row_sum(c, tpr, red[turn & 1]) / float(a.hidden);
-    ++turn;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * tpr) * 8, left = live ? a.hidden - col : 0;
-      if (left <= 0) continue;
-      float d[8], n[8], e[8], out[8];
-      unpack<T>(dy[k], d);
-      unpack<T>(h[k], n);
-      unpack<T>(dh[k], e);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) out[j] = fmaf(rstd, d[j] * w[k][j] - n[j] * rstd * c, e[j]);
-      store<T, VEC>(static_cast<T*>(a.dx) + row * a.hidden + col, out, left);
+    for (int s = 0; s < kStages; ++s) {  // the stage is a constant, so rstds stays in registers
+      if (row - slot >= a.rows) break;
+      // Into the stage of the row before, whose values this thread has used.
+      fetch((s + kStages - 1) % kStages, rstds[(s + kStages - 1) % kStages]);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      Load<T, true, K> dy, h, dh;
+      ring.read(s, 0, dy);
+      ring.read(s, 1, h);
+      if (a.dh.p) ring.read(s, 2, dh);
+      finish_grad<T, W, true, K>(a, row, row < a.rows, part, dy, h, dh, rstds[s], wv, acc, red[s & 1]);
+      row += stride;
     }
   }
-  float* to = a.partial + (long long)blockIdx.x * a.hidden;
-  if (tpr > 32) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (lane + k * tpr) * 8;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (col + j < a.hidden) to[col + j] = acc[k][j];
-    }
-  } else {  // several rows at once: add the block's slots in order
-#pragma unroll
-    for (int j = 0; j < 8; ++j) slots[threadIdx.x * 8 + j] = acc[0][j];
-    __syncthreads();
-    for (int col = threadIdx.x; col < a.hidden; col += blockDim.x) {
-      float s = 0.0f;
-      for (int q = 0; q < per; ++q) s += slots[q * tpr * 8 + col];
-      to[col] = s;
-    }
-  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  store_partial<K, true>(a, part, acc, reinterpret_cast<float*>(smem));
 }
 
 // Long rows: dx with two passes over the row (the second from L2) ...
-template <typename T, bool VEC>
+template <typename T, typename W, bool VEC>
 __global__ void __launch_bounds__(kLongThreads) norm_backward_long_kernel(const __grid_constant__ BwdArgs a) {
   __shared__ float red[32];
   const long long row = blockIdx.x;
+  const Row from(row, a.split);
   const float rstd = a.rstd[row];
-  float c = 0.0f;
-  for (int col = threadIdx.x * 8; col < a.hidden; col += kLongThreads * 8) {
-    const int left = a.hidden - col;
-    float d[8], n[8], w[8];
-    unpack<T>(load<T, VEC>(row_of<T>(a.dy, row, a.inner) + col, left), d);
-    unpack<T>(load<T, VEC>(row_of<T>(a.h, row, a.inner) + col, left), n);
-    load_weight<T, VEC>(a.weight, a.wf32, col, left, w);
+  const Pair r2 = pair(rstd, rstd);
+  const auto terms = [&](const Part<1, VEC>& part, Pair (&g)[4], Pair (&n)[4]) {
+    Load<T, VEC, 1> dy, h;
+    Load<W, VEC, 1> wv;
+    Pair w[4];
+    dy.load(from.of<T>(a.dy), part);
+    h.load(from.of<T>(a.h), part);
+    wv.load(static_cast<const W*>(a.weight), part);
+    dy.get(0, g);
+    h.get(0, n);
+    wv.get(0, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c = fmaf(d[j] * w[j], n[j] * rstd, c);
-  }
-  c = row_sum(c, kLongThreads, red) / float(a.hidden);
-  for (int col = threadIdx.x * 8; col < a.hidden; col += kLongThreads * 8) {
-    const int left = a.hidden - col;
-    float d[8], n[8], w[8], e[8] = {}, out[8];
-    unpack<T>(load<T, VEC>(row_of<T>(a.dy, row, a.inner) + col, left), d);
-    unpack<T>(load<T, VEC>(row_of<T>(a.h, row, a.inner) + col, left), n);
-    load_weight<T, VEC>(a.weight, a.wf32, col, left, w);
-    if (a.dh.p) unpack<T>(load<T, VEC>(row_of<T>(a.dh, row, a.inner) + col, left), e);
+    for (int j = 0; j < 4; ++j) {
+      n[j] = n[j] * r2;
+      g[j] = g[j] * w[j];
+    }
+  };
+  Pair sum = pair(0.0f, 0.0f);
+  each_turn<VEC>(a.hidden, [&](const Part<1, VEC>& part) {
+    if (part.left[0] <= 0) return;
+    Pair g[4], n[4];
+    terms(part, g, n);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out[j] = fmaf(rstd, d[j] * w[j] - n[j] * rstd * c, e[j]);
-    store<T, VEC>(static_cast<T*>(a.dx) + row * a.hidden + col, out, left);
-  }
+    for (int j = 0; j < 4; ++j) sum = fma(g[j], n[j], sum);
+  });
+  const float c = row_sum(sum_of(sum), kLongThreads, red) * -a.inv_hidden;
+  each_turn<VEC>(a.hidden, [&](const Part<1, VEC>& part) {
+    if (part.left[0] <= 0) return;
+    Pair g[4], n[4], e[4] = {};
+    terms(part, g, n);
+    if (a.dh.p) {
+      Load<T, VEC, 1> dh;
+      dh.load(from.of<T>(a.dh), part);
+      dh.get(0, e);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = fma(fma(n[j], pair(c, c), g[j]), r2, e[j]);
+    float f[8];
+    split(e, f);
+    store8<T, VEC>(static_cast<T*>(a.dx) + row * a.hidden + part.at[0], f, part.step, part.left[0]);
+  });
 }
 
 // ... and dw by columns: block (x, y) adds rows y, y + gridDim.y, ... of its columns.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dw_long_kernel(const __grid_constant__ BwdArgs a) {
-  const int col = (blockIdx.x * 256 + threadIdx.x) * 8, left = a.hidden - col;
-  if (left <= 0) return;
-  float acc[8] = {};
+  Part<1, VEC> part(threadIdx.x, 256, 256 * 8);
+  part.at[0] += blockIdx.x * 256 * 8;
+  part.left[0] = a.hidden - part.at[0];
+  if (part.left[0] <= 0) return;
+  Pair acc[4] = {};
   for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const Row from(row, a.split);
     const float rstd = a.rstd[row];
-    float d[8], n[8];
-    unpack<T>(load<T, VEC>(row_of<T>(a.dy, row, a.inner) + col, left), d);
-    unpack<T>(load<T, VEC>(row_of<T>(a.h, row, a.inner) + col, left), n);
+    Load<T, VEC, 1> dy, h;
+    Pair d[4], n[4];
+    dy.load(from.of<T>(a.dy), part);
+    h.load(from.of<T>(a.h), part);
+    dy.get(0, d);
+    h.get(0, n);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = fmaf(d[j], n[j] * rstd, acc[j]);
+    for (int j = 0; j < 4; ++j) acc[j] = fma(d[j], n[j] * pair(rstd, rstd), acc[j]);
   }
-  float* to = a.partial + (long long)blockIdx.y * a.hidden + col;
+  float* to = a.partial + (long long)blockIdx.y * a.hidden + part.at[0];
+  float f[8];
+  split(acc, f);
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (j < left) to[j] = acc[j];
+    if (j * part.step < part.left[0]) to[j * part.step] = f[j];
 }
 
 // dw[col] = sum of the blocks' parts: a warp-wide strip of 32 columns per
@@ -434,10 +709,14 @@ __global__ void __launch_bounds__(1024) dw_kernel(const float* partial, int part
 
 // ---------------------------------------------------------------- host
 
-// How a row is spread over threads.
+constexpr int kRingSmem = 220 * 1024;  // of an SM's shared memory, for the rings of its blocks
+
+// How rows are spread over threads and blocks.
 struct Shape {
   int tpr = 0, threads = 0, k = 0;  // k 0: the long variant
-  long long rows_per_block = 1;
+  bool ring = false;
+  size_t smem = 0;
+  long long blocks = 0;
 };
 
 int pow2_at_least(int n) {
@@ -446,76 +725,107 @@ int pow2_at_least(int n) {
   return p;
 }
 
-Shape shape_fwd(long long rows, int hidden, int sms) {
-  Shape s;
-  const int octets = (hidden + 7) / 8;
-  if (octets <= 32) {  // several rows per warp or block
-    s.tpr = pow2_at_least(octets);
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// `k` octets a thread; rows that take up to 32 threads share a block (and a warp).
+void spread(Shape& s, int octets, int k) {
+  s.k = k;
+  if (octets <= 32 * k) {
+    s.tpr = pow2_at_least(int(ceil_div(octets, k)));
     s.threads = 256;
-    s.k = 1;
-    s.rows_per_block = 256 / s.tpr;
-    return s;
+  } else {
+    s.tpr = s.threads = int(ceil_div(ceil_div(octets, 32), k)) * 32;
   }
-  if (octets > 2048) return s;
-  const int need = (octets + 31) / 32 * 32;
-  s.k = octets <= 512 || (octets <= 1024 && rows <= sms) ? 1 : octets <= 1024 ? 2 : 4;
-  s.tpr = s.threads = (need / 32 + s.k - 1) / s.k * 32;
+}
+
+long long blocks_of(const Shape& s, long long rows) {
+  return s.tpr > 32 ? rows : ceil_div(rows, s.threads / s.tpr);
+}
+
+Shape shape_fwd(long long rows, int hidden, int most, int sms) {
+  Shape s;
+  const int octets = int(ceil_div(hidden, 8));
+  s.blocks = rows;
+  if (octets > 2 * most) return s;
+  int k = octets > most || rows > sms ? 2 : 1;
+  spread(s, octets, k);
+  s.blocks = blocks_of(s, rows);
   return s;
 }
 
-Shape shape_bwd(int hidden) {
+Shape shape_bwd(long long rows, int hidden, int es, int sms) {
   Shape s;
-  const int octets = (hidden + 7) / 8;
-  if (octets <= 32) {
-    s.tpr = pow2_at_least(octets);
-    s.threads = 256;
-    s.k = 1;
-    s.rows_per_block = 256 / s.tpr;
+  const int octets = int(ceil_div(hidden, 8));
+  if (octets > 2 * kRingThreads) {  // blocks that share dw's columns
+    const long long columns = ceil_div(octets, 256), splits = ceil_div(8ll * sms, columns);
+    s.blocks = splits < rows ? splits : rows;
     return s;
   }
-  if (octets > 2048) return s;
-  s.k = octets <= 1024 ? 1 : 2;
-  s.tpr = s.threads = ((octets + 31) / 32 + s.k - 1) / s.k * 32;
+  spread(s, octets, 2);
+  // Sized for three sources, so that the parts of dw do not depend on them.
+  s.smem = size_t(kStages) * 3u * 2u * size_t(s.threads) * 16u;
+  const int by_threads = kRingThreads / s.threads, by_smem = int(size_t(kRingSmem) / s.smem);
+  s.ring = es == 2 && by_smem > 0;
+  // As many blocks as are resident, but with four rows each before every SM has more than one.
+  const long long fit = (long long)sms * (s.ring && by_smem < by_threads ? by_smem : by_threads);
+  const long long most = blocks_of(s, rows), few = ceil_div(most, 4);
+  s.blocks = most < sms ? most : few < sms ? sms : few < fit ? few : fit;
   return s;
 }
 
-// Blocks that share dw, and so the parts of the workspace.
-long long backward_blocks(long long rows, int hidden, int sms) {
-  const Shape s = shape_bwd(hidden);
-  if (!s.k) {
-    const long long columns = ((hidden + 7) / 8 + 255) / 256;
-    long long splits = (8ll * sms + columns - 1) / columns;
-    return splits < rows ? splits : rows;
+RowSplit split_by(long long inner) {
+  RowSplit s;
+  s.inner = unsigned(inner);
+  s.shift = 0;
+  while ((1ull << s.shift) < (unsigned long long)inner) ++s.shift;
+  s.magic = unsigned(((1ull << 32) * ((1ull << s.shift) - (unsigned long long)inner)) / (unsigned long long)inner + 1);
+  return s;
+}
+
+template <typename T, typename W, bool F8, bool VEC>
+const void* fwd_kernel(int k, bool many) {
+  if (k == 1) return many ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, VEC, true, 1>)
+                          : reinterpret_cast<const void*>(norm_kernel<T, W, F8, VEC, false, 1>);
+  if (k == 2) return many ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, VEC, true, 2>)
+                          : reinterpret_cast<const void*>(norm_kernel<T, W, F8, VEC, false, 2>);
+  return reinterpret_cast<const void*>(norm_long_kernel<T, W, F8, VEC>);
+}
+
+// The kernels of an input and a weight type.
+template <typename T, typename W>
+struct Kernels {
+  static const void* fwd(bool f8, bool vec, int k, bool many) {
+    if (f8) return vec ? fwd_kernel<T, W, true, true>(k, many) : fwd_kernel<T, W, true, false>(k, many);
+    return vec ? fwd_kernel<T, W, false, true>(k, many) : fwd_kernel<T, W, false, false>(k, many);
   }
-  const long long want = (rows + s.rows_per_block - 1) / s.rows_per_block;
-  const long long fit = (long long)sms * (2048 / s.threads);
-  return want < fit ? want : fit;
-}
+  static const void* bwd(bool vec, const Shape& s) {
+    if constexpr (sizeof(T) == 2)
+      if (s.k && vec && s.ring) return reinterpret_cast<const void*>(norm_backward_ring_kernel<T, W, 2>);
+    if (s.k)
+      return vec ? reinterpret_cast<const void*>(norm_backward_kernel<T, W, true, 2>)
+                 : reinterpret_cast<const void*>(norm_backward_kernel<T, W, false, 2>);
+    return vec ? reinterpret_cast<const void*>(norm_backward_long_kernel<T, W, true>)
+               : reinterpret_cast<const void*>(norm_backward_long_kernel<T, W, false>);
+  }
+};
 
-template <typename T, bool F8, bool VEC>
-const void* fwd_kernel(int k) {
-  switch (k) {
-    case 1: return reinterpret_cast<const void*>(norm_kernel<T, F8, VEC, 1>);
-    case 2: return reinterpret_cast<const void*>(norm_kernel<T, F8, VEC, 2>);
-    case 4: return reinterpret_cast<const void*>(norm_kernel<T, F8, VEC, 4>);
-    default: return reinterpret_cast<const void*>(norm_long_kernel<T, F8, VEC>);
+template <typename F>
+const void* by_types(int dtype, bool wf32, F f) {
+  switch (dtype) {
+    case NB_NORM_FLOAT32: return f(Kernels<float, float>());
+    case NB_NORM_FLOAT16: return wf32 ? f(Kernels<__half, float>()) : f(Kernels<__half, __half>());
+    default: return wf32 ? f(Kernels<__nv_bfloat16, float>()) : f(Kernels<__nv_bfloat16, __nv_bfloat16>());
   }
 }
 
-template <typename T>
-const void* pick_fwd(bool f8, bool vec, int k) {
-  if (f8) return vec ? fwd_kernel<T, true, true>(k) : fwd_kernel<T, true, false>(k);
-  return vec ? fwd_kernel<T, false, true>(k) : fwd_kernel<T, false, false>(k);
-}
-
-template <typename T>
-const void* pick_bwd(bool vec, int k) {
-  if (k == 1) return vec ? reinterpret_cast<const void*>(norm_backward_kernel<T, true, 1>)
-                         : reinterpret_cast<const void*>(norm_backward_kernel<T, false, 1>);
-  if (k == 2) return vec ? reinterpret_cast<const void*>(norm_backward_kernel<T, true, 2>)
-                         : reinterpret_cast<const void*>(norm_backward_kernel<T, false, 2>);
-  return vec ? reinterpret_cast<const void*>(norm_backward_long_kernel<T, true>)
-             : reinterpret_cast<const void*>(norm_backward_long_kernel<T, false>);
+cudaError_t launch(const void* fn, const Shape& s, bool ring, unsigned blocks, void** argv, cudaStream_t stream) {
+  size_t smem = 0;
+  if (ring) {
+    smem = s.smem;
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return e;
+  }
+  return cudaLaunchKernel(fn, dim3(blocks), dim3(unsigned(s.k ? s.threads : kLongThreads)), argv, smem, stream);
 }
 
 template <typename T>
@@ -532,6 +842,8 @@ int size_of(int dtype) {
     default: return 0;
   }
 }
+
+constexpr char kNegative[] = "bad arguments: negative stride";
 
 // Whether rows at these strides start on the boundary of an octet (element
 // alignment is checked apart).
@@ -582,44 +894,44 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   OpDevice dev(a->device);
   if (dev.error()) return op_refuse(err, errcap, "cannot use the device", int(dev.error()));
 
-  const Shape s = shape_fwd(a->rows, a->hidden, dev.sms());
   FwdArgs k{};
   bool vec = a->hidden % 8 == 0 && octets_fit(a->weight, 0, 0, size_of(a->weight_dtype));
   for (int i = 0; i < a->parts; ++i) {
+    if (a->x_outer[i] < 0 || a->x_inner[i] < 0) return op_refuse(err, errcap, kNegative);
     k.x[i] = {a->x[i], a->x_outer[i], a->x_inner[i]};
     vec = vec && octets_fit(a->x[i], a->x_outer[i], a->x_inner[i], es);
   }
+  if (a->r_outer < 0 || a->r_inner < 0) return op_refuse(err, errcap, kNegative);
   k.residual = {a->residual, a->r_outer, a->r_inner};
   if (a->residual) vec = vec && octets_fit(a->residual, a->r_outer, a->r_inner, es);
   vec = vec && octets_fit(a->y, 0, 0, f8 ? 1 : es) && (!a->h || octets_fit(a->h, 0, 0, es));
+  const Shape s = shape_fwd(a->rows, a->hidden, max_threads(vec, a->parts > 1), dev.sms());
   k.weight = a->weight;
   k.y = a->y;
   k.scale = a->scale;
   k.h = a->h;
   k.rstd = a->rstd;
   k.rows = a->rows;
-  k.inner = a->inner;
+  k.split = split_by(a->inner);
   k.hidden = a->hidden;
   k.parts = a->parts;
-  k.wf32 = a->weight_dtype == NB_NORM_FLOAT32;
   k.group = a->group;
   k.groups = a->group ? (a->hidden + a->group - 1) / a->group : 1;
-  k.tpr = s.k ? s.tpr : kLongThreads;
+  k.tpr = s.tpr;
   k.eps = a->eps;
-  const void* fn = a->dtype == NB_NORM_FLOAT32   ? pick_fwd<float>(f8, vec, s.k)
-                   : a->dtype == NB_NORM_FLOAT16 ? pick_fwd<__half>(f8, vec, s.k)
-                                                 : pick_fwd<__nv_bfloat16>(f8, vec, s.k);
+  k.inv_hidden = 1.0f / float(a->hidden);
+  const void* fn = by_types(a->dtype, a->weight_dtype == NB_NORM_FLOAT32,
+                            [&](auto kernels) { return kernels.fwd(f8, vec, s.k, a->parts > 1); });
   void* argv[] = {&k};
-  const unsigned blocks = unsigned((a->rows + s.rows_per_block - 1) / s.rows_per_block);
-  const cudaError_t e = cudaLaunchKernel(fn, dim3(blocks), dim3(s.k ? s.threads : kLongThreads), argv, 0,
-                                         static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch(fn, s, false, unsigned(s.blocks), argv, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : op_refuse(err, errcap, "launch of the norm failed", int(e));
 }
 
-extern "C" uint64_t nb_add_rms_norm_backward_workspace(int device, int64_t rows, int hidden) {
+extern "C" uint64_t nb_add_rms_norm_backward_workspace(int device, int64_t rows, int hidden, int dtype) {
+  const int es = size_of(dtype);
   OpDevice dev(device);
-  if (dev.error() || rows < 0 || hidden < 1) return 0;
-  return uint64_t(backward_blocks(rows, hidden, dev.sms())) * uint64_t(hidden) * sizeof(float);
+  if (dev.error() || rows < 0 || hidden < 1 || !es) return 0;
+  return uint64_t(shape_bwd(rows, hidden, es, dev.sms()).blocks) * uint64_t(hidden) * sizeof(float);
 }
 
 extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, char* err, size_t errcap) {
@@ -634,12 +946,14 @@ extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, c
     return op_refuse(err, errcap, "bad arguments: null or misaligned tensor");
   OpDevice dev(a->device);
   if (dev.error()) return op_refuse(err, errcap, "cannot use the device", int(dev.error()));
-  const long long parts = backward_blocks(a->rows, a->hidden, dev.sms());
+  const Shape s = shape_bwd(a->rows, a->hidden, es, dev.sms());
+  const long long parts = s.blocks;
   if (a->rows && (misplaced(a->workspace, 4) || a->workspace_bytes < uint64_t(parts) * uint64_t(a->hidden) * 4))
     return op_refuse(err, errcap, "bad arguments: the workspace is too small");
 
-  const Shape s = shape_bwd(a->hidden);
   BwdArgs k{};
+  if (a->dy_outer < 0 || a->dy_inner < 0 || a->h_outer < 0 || a->h_inner < 0 || a->dh_outer < 0 || a->dh_inner < 0)
+    return op_refuse(err, errcap, kNegative);
   k.dy = {a->dy, a->dy_outer, a->dy_inner};
   k.h = {a->h, a->h_outer, a->h_inner};
   k.dh = {a->dh, a->dh_outer, a->dh_inner};
@@ -648,10 +962,10 @@ extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, c
   k.dx = a->dx;
   k.partial = a->workspace;
   k.rows = a->rows;
-  k.inner = a->inner;
+  k.split = split_by(a->inner);
   k.hidden = a->hidden;
-  k.wf32 = a->weight_dtype == NB_NORM_FLOAT32;
   k.tpr = s.tpr;
+  k.inv_hidden = 1.0f / float(a->hidden);
   const bool vec = a->hidden % 8 == 0 && octets_fit(a->weight, 0, 0, ws) &&
                    octets_fit(a->dy, a->dy_outer, a->dy_inner, es) && octets_fit(a->h, a->h_outer, a->h_inner, es) &&
                    (!a->dh || octets_fit(a->dh, a->dh_outer, a->dh_inner, es)) && octets_fit(a->dx, 0, 0, es);
@@ -659,11 +973,9 @@ extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, c
   void* argv[] = {&k};
   cudaError_t e = cudaSuccess;
   if (a->rows) {
-    const void* fn = a->dtype == NB_NORM_FLOAT32   ? pick_bwd<float>(vec, s.k)
-                     : a->dtype == NB_NORM_FLOAT16 ? pick_bwd<__half>(vec, s.k)
-                                                   : pick_bwd<__nv_bfloat16>(vec, s.k);
-    const unsigned blocks = unsigned(s.k ? parts : a->rows);
-    e = cudaLaunchKernel(fn, dim3(blocks), dim3(s.k ? s.threads : kLongThreads), argv, 0, st);
+    const void* fn = by_types(a->dtype, a->weight_dtype == NB_NORM_FLOAT32,
+                              [&](auto kernels) { return kernels.bwd(vec, s); });
+    e = launch(fn, s, s.ring && vec, unsigned(s.k ? parts : a->rows), argv, st);
     if (e == cudaSuccess && !s.k) {
       fn = a->dtype == NB_NORM_FLOAT32   ? pick_dw_long<float>(vec)
            : a->dtype == NB_NORM_FLOAT16 ? pick_dw_long<__half>(vec)

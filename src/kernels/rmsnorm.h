@@ -54,6 +54,6 @@ struct nb_norm_grad_t {
   int32_t device, hidden, dtype, weight_dtype;
 };
 int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, char* err, size_t errcap);
-// Bytes of workspace for these sizes on `device` (a bound for every stride and alignment).
-uint64_t nb_add_rms_norm_backward_workspace(int device, int64_t rows, int hidden);
+// Bytes of workspace for these sizes on `device`, whatever the strides and alignment.
+uint64_t nb_add_rms_norm_backward_workspace(int device, int64_t rows, int hidden, int dtype);
 }

@@ -8,37 +8,38 @@ import pytest
 CHUNK = 2048
 
 
-def pack(core, sizes, room):
+def pack(core, sizes, room, chunk=CHUNK):
     L = core.lib()
-    L.nb_pack_tensors.argtypes = [C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]
+    L.nb_pack_tensors.argtypes = [C.c_void_p, C.c_size_t, C.c_int, C.c_uint, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]
     n = len(sizes)
     arr = (C.c_uint64 * n)(*sizes)
     out = []
-    for k in range(L.nb_pack_tensors(arr, n, room, -1, None, None, None)):
+    for k in range(L.nb_pack_tensors(arr, n, room, chunk, -1, None, None, None)):
         tensor, first, chunks = (C.c_int * n)(), (C.c_uint * n)(), C.c_uint()
-        m = L.nb_pack_tensors(arr, n, room, k, tensor, first, C.byref(chunks))
+        m = L.nb_pack_tensors(arr, n, room, chunk, k, tensor, first, C.byref(chunks))
         out.append((list(tensor)[:m], list(first)[:m], chunks.value))
     return out
 
 
+@pytest.mark.parametrize("chunk", [2048, 8192])
 @pytest.mark.parametrize("room", [1, 2, 7, 400])
-def test_every_chunk_finds_its_tensor(core, room):
+def test_every_chunk_finds_its_tensor(core, room, chunk):
     rng = random.Random(room)
-    sizes = [rng.choice([0, 1, 2047, 2048, 2049, rng.randrange(1, 50000)]) for _ in range(60)]
+    sizes = [rng.choice([0, 1, 2047, 2048, 2049, 8192, 8193, rng.randrange(1, 50000)]) for _ in range(60)]
     L = core.lib()
     L.nb_find_tensor.argtypes = [C.c_uint, C.c_void_p, C.c_int]
     covered = {}
-    for tensor, first, chunks in pack(core, sizes, room):
+    for tensor, first, chunks in pack(core, sizes, room, chunk):
         assert 1 <= len(tensor) <= room and first[0] == 0
         arr = (C.c_uint * len(first))(*first)
         for c in range(chunks):
             i = L.nb_find_tensor(c, arr, len(first))
             assert first[i] <= c and (i + 1 == len(first) or c < first[i + 1])
-            begin = (c - first[i]) * CHUNK
+            begin = (c - first[i]) * chunk
             assert begin < sizes[tensor[i]]
             covered.setdefault(tensor[i], []).append(begin)
     for i, n in enumerate(sizes):
-        assert sorted(covered.get(i, [])) == list(range(0, n, CHUNK))
+        assert sorted(covered.get(i, [])) == list(range(0, n, chunk))
 
 
 def test_empty_and_huge_lists(core):

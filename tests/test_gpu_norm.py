@@ -105,6 +105,27 @@ def test_partials(parts, residual, dtype):
         check(m.add_rms_norm(xs, w, res, eps=1e-5, out_dtype=E4M3, group=128), xs, w, res, 1e-5, 128)
 
 
+# Many rows: blocks that walk over them, at each row width's number of threads.
+MANY = [(40000, 8), (30001, 24), (20001, 128), (9000, 256), (5003, 264), (3001, 1024), (2500, 2048), (1300, 4096),
+        (700, 5120), (1000, 8192), (650, 16384)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows, hidden", MANY)
+def test_many_rows(rows, hidden, dtype):
+    m = norm()
+    xs = [data((rows, hidden), dtype, k) for k in range(2)]
+    res, w = data((rows, hidden), dtype, 5, 2.0), data((hidden,), torch.float32, 3)
+    check(m.add_rms_norm(xs[0], w, res), xs[:1], w, res, 1e-6)
+    check(m.add_rms_norm(xs, w.to(dtype)), xs, w.to(dtype), None, 1e-6)
+    for group in (0, 128):
+        check(m.add_rms_norm(xs, w, res, out_dtype=E4M3, group=group), xs, w, res, 1e-6, group)
+    # in place, where rows are fetched ahead of the row that is written
+    want = m.add_rms_norm(xs, w, res)
+    got = m.add_rms_norm(xs, w, res, out=m.NormOut(torch.empty_like(res), None, res, torch.empty_like(want.rstd)))
+    assert torch.equal(got.y, want.y) and torch.equal(res, want.h)
+
+
 def test_sum_has_the_bits_of_the_collectives_fold():
     m = norm()
     from scc26_nccl_shim_b200.ops import emu
@@ -252,7 +273,7 @@ def grad_reference(dy, h, w, rstd, dh):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("rows, hidden", SHAPES + [(1, 4096), (2500, 128), (700, 2048), (9, 17000)])
+@pytest.mark.parametrize("rows, hidden", SHAPES + MANY + [(1, 4096), (9, 17000)])
 def test_gradient(rows, hidden, dtype):
     m = norm()
     h, dy = data((rows, hidden), dtype, 1, 2.0), data((rows, hidden), dtype, 2)
