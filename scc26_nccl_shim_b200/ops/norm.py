@@ -26,9 +26,9 @@ E4M3 = torch.float8_e4m3fn
 NCCL_E4M3 = 10
 GROUPS = (0, 32, 64, 128)
 
-_FWD = struct.Struct("8Q8q8qQ2q5Q2q7if")       # nb_norm_t
+# nb_norm_t, by the number of partial sums (the arrays' other places are zero)
+_FWD = [struct.Struct(f"{n}Q{8 * (8 - n)}x{n}q{8 * (8 - n)}x{n}q{8 * (8 - n)}xQ2q5Q2q7if") for n in range(9)]
 _BWD = struct.Struct("Q2qQ2qQ2qQQQQQQ2q4i")    # nb_norm_grad_t
-_PAD = [(0,) * (8 - n) for n in range(9)]
 _ERR = 256
 
 
@@ -58,14 +58,14 @@ def _workspace_bytes(device: int, rows: int, hidden: int, dtype: int) -> int:
     return int(lib().nb_add_rms_norm_backward_workspace(device, rows, hidden, dtype))
 
 
-def _strides(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+def _strides(t: torch.Tensor) -> tuple[int, int, int]:
     """(inner, outer stride, inner stride): row r of `t` starts at
     (r // inner) * outer stride + (r % inner) * inner stride elements."""
     hidden = t.shape[-1]
     if t.is_contiguous():
         return 1, hidden, 0
     if t.stride(-1) != 1 and hidden > 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
+        raise ValueError("the last dimension must be contiguous")
     dims: list[list[int]] = []  # [size, stride], neighbours merged
     for n, s in zip(t.shape[:-1], t.stride()[:-1]):
         if n == 1:
@@ -80,24 +80,27 @@ def _strides(t: torch.Tensor, name: str) -> tuple[int, int, int]:
         return 1, dims[0][1], 0
     if len(dims) == 2:
         return dims[1][0], dims[0][1], dims[1][1]
-    raise ValueError(f"{name}: rows at more than two different strides (call .contiguous())")
+    raise ValueError("rows at more than two different strides (call .contiguous())")
 
 
-def _rows(ts: Sequence[tuple[torch.Tensor, str]]) -> tuple[int, list[tuple[int, int]]]:
-    """The split of the row number that all of these share, and their strides."""
-    hidden = ts[0][0].shape[-1]
-    if all([t.is_contiguous() for t, _ in ts]):
-        return 1, [(hidden, 0)] * len(ts)
-    got = [_strides(t, name) for t, name in ts]
+def _rows(ts: Sequence[torch.Tensor]) -> tuple[int, list[int], list[int]]:
+    """The split of the row number that all of these share (its inner size),
+    and each one's outer and inner strides."""
+    for t in ts:
+        if not t.is_contiguous():
+            break
+    else:
+        return 1, [ts[0].shape[-1]] * len(ts), [0] * len(ts)
+    got = [_strides(t) for t in ts]
     inner = 1
-    for (n, _, _), (_, name) in zip(got, ts):
+    for n, _, _ in got:
         if n != 1:
             if inner != 1 and inner != n:
-                raise ValueError(f"{name}: rows are split unlike the other tensors' (call .contiguous())")
+                raise ValueError("the tensors' rows are split at different places (call .contiguous())")
             inner = n
     if inner == 1:
-        return 1, [(o, i) for _, o, i in got]
-    return inner, [(o, i) if n != 1 else (inner * o, o) for n, o, i in got]
+        return 1, [o for _, o, _ in got], [i for _, _, i in got]
+    return inner, [o if n != 1 else inner * o for n, o, _ in got], [i if n != 1 else o for n, o, i in got]
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -112,15 +115,16 @@ def _disjoint(a: torch.Tensor, b: torch.Tensor) -> bool:
     return e <= p or q <= s
 
 
-def _check_weight(weight: torch.Tensor, hidden: int, dtype: torch.dtype, device: torch.device) -> None:
+def _check_weight(weight: torch.Tensor, hidden: int, dtype: torch.dtype, device: torch.device) -> int:
     if weight.dim() != 1 or weight.shape[0] != hidden:
         raise ValueError(f"weight: expected shape ({hidden},), got {tuple(weight.shape)}")
     if weight.dtype != dtype and weight.dtype != torch.float32:
         raise TypeError(f"weight: expected {dtype} or torch.float32, got {weight.dtype}")
-    if weight.stride(0) != 1 and hidden > 1:
+    if not weight.is_contiguous():
         raise ValueError("weight: must be contiguous")
     if weight.device != device:
         raise ValueError(f"weight: on {weight.device}, the input on {device}")
+    return DTYPE[weight.dtype]
 
 
 def _like(t: torch.Tensor, ref: torch.Tensor, name: str) -> None:
@@ -132,17 +136,8 @@ def _like(t: torch.Tensor, ref: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: on {t.device}, expected {ref.device}")
 
 
-def _on_gpu(t: torch.Tensor) -> int:
-    if not t.is_cuda:
-        raise ValueError(f"the tensors must be on a CUDA device, got {t.device}")
-    return t.device.index
-
-
-def _run(fn, packed: bytes, device: int) -> None:
-    err = C.create_string_buffer(_ERR)
-    rc = fn(packed, emu.raw_stream(device), err, _ERR)
-    if rc:
-        raise RuntimeError(f"{err.value.decode()} ({rc})")
+def _raise(err, rc: int) -> None:
+    raise RuntimeError(f"{err.value.decode()} ({rc})")
 
 
 def _empty(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
@@ -175,54 +170,57 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
     x_0 itself, nothing else may overlap).
     """
     xs = [x] if isinstance(x, torch.Tensor) else list(x)
-    if not 1 <= len(xs) <= 8:
-        raise ValueError(f"1 to 8 partial sums, got {len(xs)}")
+    n = len(xs)
+    if not 1 <= n <= 8:
+        raise ValueError(f"1 to 8 partial sums, got {n}")
     x0 = xs[0]
-    dtype, shape = x0.dtype, x0.shape
-    if dtype not in DTYPE:
+    dtype, shape, dev = x0.dtype, x0.shape, x0.device
+    code = DTYPE.get(dtype)
+    if code is None:
         raise TypeError(f"x: expected fp16, bf16 or fp32, got {dtype}")
-    if x0.dim() < 1 or shape[-1] < 1:
+    if not shape or shape[-1] < 1:
         raise ValueError(f"x: expected shape [..., hidden] with hidden >= 1, got {tuple(shape)}")
-    hidden = shape[-1]
-    for i in range(1, len(xs)):
-        _like(xs[i], x0, f"x[{i}]")
-    if residual is not None:
-        _like(residual, x0, "residual")
-    _check_weight(weight, hidden, dtype, x0.device)
-    f8 = out_dtype == E4M3
-    if not f8 and out_dtype is not None and out_dtype != dtype:
+    hidden, lead = shape[-1], shape[:-1]
+    sources = xs if residual is None else xs + [residual]
+    for t in sources[1:]:
+        if t.dtype != dtype or t.shape != shape or t.device != dev:
+            _like(t, x0, "residual" if t is residual else "x")
+    wcode = _check_weight(weight, hidden, dtype, dev)
+    if out_dtype is None or out_dtype == dtype:
+        f8, ydtype, ycode = False, dtype, code
+    elif out_dtype == E4M3:
+        f8, ydtype, ycode = True, E4M3, NCCL_E4M3
+    else:
         raise TypeError(f"out_dtype: expected {dtype} or {E4M3}, got {out_dtype}")
     if group not in GROUPS or (group and not f8):
         raise ValueError(f"group: one of {GROUPS} with e4m3 output, else 0, got {group}")
     if not 0 < eps < math.inf:
         raise ValueError(f"eps: must be positive, got {eps}")
-    named = [(t, "x") for t in xs]
-    if residual is not None:
-        named.append((residual, "residual"))
-    inner, strides = _rows(named)
-    lead = shape[:-1]
-    sums = len(xs) > 1 or residual is not None
+    inner, outers, inners = _rows(sources)
+    sums = len(sources) > 1
     groups = -(-hidden // group) if group else 1
-    ydtype = E4M3 if f8 else dtype
     if out is not None:
         y, scale, h, rstd = _check_out(out, xs, weight, residual, ydtype, lead + (groups,) if f8 else None)
-    device = _on_gpu(x0)
+    if dev.type != "cuda":
+        raise ValueError(f"the tensors must be on a CUDA device, got {dev}")
+    device = dev.index
     if out is None:
-        dev = x0.device
         y = _empty(shape, ydtype, dev)
         scale = _empty(lead + (groups,), torch.float32, dev) if f8 else None
         h = _empty(shape, dtype, dev) if sums else x0
         rstd = _empty(lead, torch.float32, dev)
-    rows = rstd.numel()
-    n = len(xs)
-    pad = _PAD[n]
-    r = (residual.data_ptr(), *strides[n]) if residual is not None else (0, 0, 0)
-    _run(lib().nb_add_rms_norm,
-         _FWD.pack(*[t.data_ptr() for t in xs], *pad, *[o for o, _ in strides[:n]], *pad,
-                   *[i for _, i in strides[:n]], *pad, *r, weight.data_ptr(), y.data_ptr(),
-                   scale.data_ptr() if f8 else 0, h.data_ptr() if h is not x0 or sums else 0, rstd.data_ptr(),
-                   rows, inner, device, hidden, n, DTYPE[dtype], DTYPE[weight.dtype],
-                   NCCL_E4M3 if f8 else DTYPE[dtype], group, eps), device)
+    if residual is None:
+        r = (0, 0, 0)
+    else:
+        r = (residual.data_ptr(), outers[n], inners[n])
+    err = C.create_string_buffer(_ERR)
+    rc = lib().nb_add_rms_norm(
+        _FWD[n].pack(*[t.data_ptr() for t in xs], *outers[:n], *inners[:n], *r, weight.data_ptr(), y.data_ptr(),
+                     scale.data_ptr() if f8 else 0, h.data_ptr() if sums or h is not x0 else 0, rstd.data_ptr(),
+                     rstd.numel(), inner, device, hidden, n, code, wcode, ycode, group, eps),
+        emu.raw_stream(device), err, _ERR)
+    if rc:
+        _raise(err, rc)
     return NormOut(y, scale, h, rstd)
 
 
@@ -262,30 +260,37 @@ def add_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
     rows of dy * n, in the weight's type, added in an order that depends on
     the sizes alone. `h` and `rstd` are add_rms_norm's; dy, h and dh have one type.
     """
-    if h.dtype not in DTYPE:
-        raise TypeError(f"h: expected fp16, bf16 or fp32, got {h.dtype}")
-    if h.dim() < 1 or h.shape[-1] < 1:
-        raise ValueError(f"h: expected shape [..., hidden] with hidden >= 1, got {tuple(h.shape)}")
-    hidden = h.shape[-1]
-    _like(dy, h, "dy")
-    if dh is not None:
+    dtype, shape, dev = h.dtype, h.shape, h.device
+    code = DTYPE.get(dtype)
+    if code is None:
+        raise TypeError(f"h: expected fp16, bf16 or fp32, got {dtype}")
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"h: expected shape [..., hidden] with hidden >= 1, got {tuple(shape)}")
+    hidden = shape[-1]
+    if dy.dtype != dtype or dy.shape != shape or dy.device != dev:
+        _like(dy, h, "dy")
+    if dh is not None and (dh.dtype != dtype or dh.shape != shape or dh.device != dev):
         _like(dh, h, "dh")
-    _check_weight(weight, hidden, h.dtype, h.device)
-    if rstd.dtype != torch.float32 or rstd.shape != h.shape[:-1] or not rstd.is_contiguous():
-        raise ValueError(f"rstd: expected {tuple(h.shape[:-1])} of torch.float32, contiguous")
-    if rstd.device != h.device:
-        raise ValueError(f"rstd: on {rstd.device}, expected {h.device}")
-    named = [(dy, "dy"), (h, "h")] + ([(dh, "dh")] if dh is not None else [])
-    inner, strides = _rows(named)
-    device = _on_gpu(h)
-    rows = rstd.numel()
-    dx = _empty(h.shape, h.dtype, h.device)
-    dw = _empty((hidden,), weight.dtype, h.device)
-    nbytes = _workspace_bytes(device, rows, hidden, DTYPE[h.dtype])
-    ws = _empty((nbytes // 4,), torch.float32, h.device)
-    s = (dh.data_ptr(), *strides[2]) if dh is not None else (0, 0, 0)
-    _run(lib().nb_add_rms_norm_backward,
-         _BWD.pack(dy.data_ptr(), *strides[0], h.data_ptr(), *strides[1], *s, weight.data_ptr(), rstd.data_ptr(),
-                   dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes, rows, inner, device, hidden,
-                   DTYPE[h.dtype], DTYPE[weight.dtype]), device)
+    wcode = _check_weight(weight, hidden, dtype, dev)
+    if rstd.dtype != torch.float32 or rstd.shape != shape[:-1] or not rstd.is_contiguous():
+        raise ValueError(f"rstd: expected {tuple(shape[:-1])} of torch.float32, contiguous")
+    if rstd.device != dev:
+        raise ValueError(f"rstd: on {rstd.device}, expected {dev}")
+    inner, outers, inners = _rows([dy, h] if dh is None else [dy, h, dh])
+    if dev.type != "cuda":
+        raise ValueError(f"the tensors must be on a CUDA device, got {dev}")
+    device, rows = dev.index, rstd.numel()
+    dx = _empty(shape, dtype, dev)
+    dw = _empty((hidden,), weight.dtype, dev)
+    nbytes = _workspace_bytes(device, rows, hidden, code)
+    ws = _empty((nbytes // 4,), torch.float32, dev)
+    s = (dh.data_ptr(), outers[2], inners[2]) if dh is not None else (0, 0, 0)
+    err = C.create_string_buffer(_ERR)
+    rc = lib().nb_add_rms_norm_backward(
+        _BWD.pack(dy.data_ptr(), outers[0], inners[0], h.data_ptr(), outers[1], inners[1], *s, weight.data_ptr(),
+                  rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes, rows, inner, device, hidden,
+                  code, wcode),
+        emu.raw_stream(device), err, _ERR)
+    if rc:
+        _raise(err, rc)
     return dx, dw

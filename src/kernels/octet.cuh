@@ -14,6 +14,12 @@
 namespace nb {
 namespace octet {
 
+// For a kernel that was launched while the stream's previous one was running:
+// returns when that one has ended and its stores are visible. The previous one
+// calls op_nearly_done() when only its last stores are left.
+__device__ __forceinline__ void op_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void op_nearly_done() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 constexpr float kE4m3Max = 448.0f;
 // The least scale of a group of 8-bit values (2^-126): its reciprocal is finite.
 constexpr float kLeastScale = 1.17549435e-38f;

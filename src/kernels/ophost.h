@@ -52,4 +52,19 @@ class OpDevice {
   bool switched_ = false;
 };
 
+// Launches a kernel that begins with op_wait_for_previous(): its blocks may be
+// set up while the stream's previous kernel ends.
+inline cudaError_t op_launch_after(const void* fn, dim3 grid, dim3 block, void** argv, cudaStream_t stream) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, fn, argv);
+}
+
 }  // namespace nb

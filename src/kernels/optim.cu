@@ -307,10 +307,38 @@ __device__ __forceinline__ double warp_sum(double s) {
   return s;
 }
 
+template <typename G, bool VEC>
+struct NormRaw {
+  Oct<G> o[kNormOctets];
+  __device__ __forceinline__ void load(const G* p, int lane, long long) {
+#pragma unroll
+    for (int u = 0; u < kNormOctets; ++u) o[u] = load_oct(p + u * 256 + lane * 8);
+  }
+  __device__ __forceinline__ void get(int u, float (&f)[8]) const { unpack<G>(o[u], f); }
+};
+
+template <typename G>
+struct NormRaw<G, false> {
+  G e[kNormOctets][8];
+  __device__ __forceinline__ void load(const G* p, int lane, long long left) {
+#pragma unroll
+    for (int u = 0; u < kNormOctets; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = u * 256 + j * 32 + lane;
+        e[u][j] = at < left ? p[at] : from_float<G>(0.0f);
+      }
+  }
+  __device__ __forceinline__ void get(int u, float (&f)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = to_float<G>(e[u][j]);
+  }
+};
+
 // Squares of eight elements are added in fp32 and those sums in fp64: the
 // result does not depend on how many elements there are.
 template <typename G, int WORDS>
-__global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_constant__ GradArgs<WORDS> a) {
+__global__ void __launch_bounds__(kThreads, 4) grad_norm_kernel(const __grid_constant__ GradArgs<WORDS> a) {
   __shared__ double sums[kThreads / 32];
   const GradEntry* entries = reinterpret_cast<const GradEntry*>(a.words);
   const unsigned long long* grads = a.words + (size_t)a.count * kGradEntryWords;
@@ -325,23 +353,20 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
     if (base >= e.size) continue;
     const long long left = (long long)(e.size - base);
     const unsigned long long* from = grads + (size_t)i * a.parts;
-    if (e.vec && left >= 256 * kNormOctets) {
-      Oct<G> o[kNormOctets];
+    // Octets of neighbours, or single elements 32 apart; either way all of a
+    // part's loads are issued before the first is used.
+    const auto add = [&](auto raw) {
       float g[kNormOctets][8];
-      const G* p = reinterpret_cast<const G*>(from[0]) + base + lane * 8;
+      raw.load(reinterpret_cast<const G*>(from[0]) + base, lane, left);
 #pragma unroll
-      for (int u = 0; u < kNormOctets; ++u) o[u] = load_oct(p + u * 256);
-#pragma unroll
-      for (int u = 0; u < kNormOctets; ++u) unpack<G>(o[u], g[u]);
+      for (int u = 0; u < kNormOctets; ++u) raw.get(u, g[u]);
 #pragma unroll 1
       for (int k = 1; k < a.parts; ++k) {
-        p = reinterpret_cast<const G*>(from[k]) + base + lane * 8;
-#pragma unroll
-        for (int u = 0; u < kNormOctets; ++u) o[u] = load_oct(p + u * 256);
+        raw.load(reinterpret_cast<const G*>(from[k]) + base, lane, left);
 #pragma unroll
         for (int u = 0; u < kNormOctets; ++u) {
           float f[8];
-          unpack<G>(o[u], f);
+          raw.get(u, f);
 #pragma unroll
           for (int j = 0; j < 8; ++j) g[u][j] += f[j];
         }
@@ -353,27 +378,11 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
         for (int j = 0; j < 8; ++j) s = fmaf(g[u][j], g[u][j], s);
         total += double(s);
       }
-    } else {
-#pragma unroll 1
-      for (int u = 0; u < kNormOctets && u * 256 < left; ++u) {
-        float g[8], s = 0.0f;
-        const unsigned long long at = base + u * 256;
-        const long long rest = left - u * 256;
-        const bool vec = e.vec && rest >= 256;
-        load8<G>(reinterpret_cast<const G*>(from[0]), at, lane, rest, vec, g);
-#pragma unroll 1
-        for (int k = 1; k < a.parts; ++k) {
-          float f[8];
-          load8<G>(reinterpret_cast<const G*>(from[k]), at, lane, rest, vec, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) g[j] += f[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s = fmaf(g[j], g[j], s);
-        total += double(s);
-      }
-    }
+    };
+    if (e.vec && left >= 256 * kNormOctets) add(NormRaw<G, true>());
+    else add(NormRaw<G, false>());
   }
+  op_nearly_done();
   total = warp_sum(total);
   if (lane == 0) sums[warp] = total;
   __syncthreads();
@@ -387,6 +396,7 @@ __global__ void __launch_bounds__(1024) grad_norm_end_kernel(const double* parti
                                                              double scale, float* out) {
   __shared__ double sums[32];
   double s = 0.0;
+  op_wait_for_previous();
   for (int k = threadIdx.x; k < count; k += 1024) s += partial[k];
   s = warp_sum(s);
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
@@ -722,8 +732,8 @@ extern "C" int nb_grad_norm(const void* handle, double max_norm, double scale, f
   int count = h->partials;
   double limit = max_norm;
   void* argv[] = {&partial, &count, &limit, &scale, &out};
-  const cudaError_t e = cudaLaunchKernel(reinterpret_cast<const void*>(grad_norm_end_kernel), dim3(1), dim3(1024),
-                                         argv, 0, st);
+  const cudaError_t e =
+      op_launch_after(reinterpret_cast<const void*>(grad_norm_end_kernel), dim3(1), dim3(1024), argv, st);
   return e == cudaSuccess ? 0 : op_refuse(err, errcap, "launch of the gradient norm failed", int(e));
 }
 

@@ -27,9 +27,11 @@ namespace {
 using namespace octet;
 
 constexpr int kLongThreads = 1024;
-constexpr int kRingThreads = 512;
-// Threads of a norm's block at most: 64 registers do for one aligned sum and its residual.
-__host__ __device__ constexpr int max_threads(bool vec, bool many) { return vec && !many ? 1024 : 512; }
+constexpr int kRingThreads = 512;    // a block of the gradient's kernels at most (128 registers each)
+constexpr int kStagedThreads = 640;  // of its staged form (102 registers): two blocks an SM for up to 5120 columns
+constexpr int kAll = 1 << 30;  // as what is left of a row: a store to shared memory that has room for everything
+// A block of the norm's at most: 64 registers do for one sum and its residual.
+__host__ __device__ constexpr int max_threads(bool many) { return many ? 512 : 1024; }
 
 struct Rows {
   const void* p;
@@ -53,6 +55,7 @@ struct FwdArgs {
   long long rows;
   RowSplit split;
   int hidden, parts, group, tpr, groups;
+  int window, windows;  // elements between staged rows, and a row's number of them
   float eps, inv_hidden;
 };
 
@@ -65,6 +68,7 @@ struct BwdArgs {
   long long rows;
   RowSplit split;
   int hidden, tpr;
+  int window;  // elements between staged rows
   float inv_hidden;
 };
 
@@ -109,26 +113,31 @@ __device__ __forceinline__ uint32_t row_max(uint32_t m, int tpr, uint32_t* red) 
 }
 
 // A thread's K times eight elements of a row: where the first of each eight
-// is, how far apart they are, and how much of the row is left from there on.
-// The k-th eight of a warp's 32 threads (of a row's `tpr`, if fewer) are 256
-// (8 tpr) neighbours; each thread has eight of them in a row (VEC), or every
-// 32nd (tpr-th). Without any (left <= 0) it reads the row's first ones and
-// drops them.
+// is, and how much of the row is left from there on. The k-th eight of a
+// warp's 32 threads (of a row's `tpr`, if fewer) are 256 (8 tpr) neighbours.
+// VEC: a thread has eight of them in a row; without any (left <= 0) it reads
+// the row's first ones and drops them. Otherwise it has every 32nd.
 template <int K, bool VEC>
 struct Part {
-  int lane, step, at[K], left[K];
+  static constexpr int kStep = VEC ? 1 : 32;
+  int lane, at[K], left[K];
 
   __device__ __forceinline__ Part(int lane_, int tpr, int hidden) : lane(lane_) {
-    const int width = tpr < 32 ? tpr : 32, in = lane & (width - 1);
-    step = VEC ? 1 : width;
+    const int in = lane & 31;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      at[k] = (lane - in + k * tpr) * 8 + (VEC ? in * 8 : in);
+      at[k] = VEC ? (lane + k * tpr) * 8 : (lane - in + k * tpr) * 8 + in;
       left[k] = hidden - at[k];
-      if (left[k] <= 0) at[k] = 0;
+      if (VEC && left[k] <= 0) at[k] = 0;
     }
   }
 };
+
+// The threads of one row: a warp's, or the block's.
+__device__ __forceinline__ void row_sync(int tpr) {
+  if (tpr > 32) __syncthreads();
+  else __syncwarp();
+}
 
 // A thread's elements of one row of a tensor.
 template <typename T, bool VEC, int K>
@@ -137,7 +146,7 @@ struct Load {
 
   __device__ __forceinline__ void load(const T* row, const Part<K, VEC>& part) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) raw[k].load(row + part.at[k], part.step, part.left[k]);
+    for (int k = 0; k < K; ++k) raw[k].load(row + part.at[k], part.kStep, part.left[k]);
   }
   __device__ __forceinline__ void get(int k, Pair (&f)[4]) const { raw[k].get(f); }
 };
@@ -175,17 +184,16 @@ __device__ __forceinline__ float reciprocal(float scale) { return __fdividef(1.0
 
 // The reciprocals of the scales of groups of 32, 64 or 128 columns, one for each
 // of a thread's eight values; the group's first thread stores its scale. `whole`: the
-// largest magnitude of the row's part, where a group is wider than that.
+// largest magnitude of a thread's part, where a group is wider than the row's threads.
 template <bool VEC>
 __device__ __forceinline__ void group_scales(const FwdArgs& a, const float (&y)[8], uint32_t whole, int tpr,
                                              long long row, int at, int left, float (&inv)[8]) {
-  const int width = tpr < 32 ? tpr : 32;
   float* to = a.scale + row * a.groups;
   if constexpr (VEC) {  // a thread's values are in one group, with its neighbours
     uint32_t top = left > 0 ? top_of(y) : 0;
     int lanes = a.group >> 3;
-    if (lanes > width) {
-      lanes = width;
+    if (lanes > tpr) {
+      lanes = tpr;
       top = whole;
     }
     for (int o = lanes >> 1; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
@@ -193,18 +201,13 @@ __device__ __forceinline__ void group_scales(const FwdArgs& a, const float (&y)[
     if (left > 0 && (at & (a.group - 1)) == 0) to[unsigned(at) / unsigned(a.group)] = s;
 #pragma unroll
     for (int j = 0; j < 8; ++j) inv[j] = i;
-  } else {  // a group is `per` neighbouring j of all the row's lanes
-    const int per = a.group / width;
+  } else {  // a group is one, two or four neighbouring j of a warp's lanes
     uint32_t top[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top[j] = j * width < left ? magnitude(y[j]) : 0;
-    if (per > 8) {
+    for (int j = 0; j < 8; ++j) top[j] = j * 32 < left ? magnitude(y[j]) : 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top[j] = whole;
-    }
-#pragma unroll
-    for (int half = 1; half < 8; half *= 2)
-      if (per > half) {
+    for (int half = 1; half < 4; half *= 2)
+      if (a.group > 32 * half) {
         uint32_t other[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) other[j] = top[j ^ half];
@@ -213,33 +216,197 @@ __device__ __forceinline__ void group_scales(const FwdArgs& a, const float (&y)[
       }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      for (int o = width >> 1; o; o >>= 1) top[j] = max(top[j], __shfl_xor_sync(~0u, top[j], o));
-      const float s = scale_of(top[j]);
+      const float s = scale_of(__reduce_max_sync(~0u, top[j]));
       inv[j] = reciprocal(s);
-      const int col = at + j * width;
-      if (j * width < left && (col & (a.group - 1)) == 0) to[unsigned(col) / unsigned(a.group)] = s;
+      const int col = at + j * 32;
+      if (j * 32 < left && (col & (a.group - 1)) == 0) to[unsigned(col) / unsigned(a.group)] = s;
     }
+  }
+}
+
+// A row off the vector boundary as it lies in shared memory: the aligned
+// 16-byte pieces that hold it, copied asynchronously by the row's threads. What a
+// piece holds before the row is the tensor's own (the row's element 0 is at
+// `shift` elements); behind the row's end nothing is read.
+template <typename T>
+struct Window {
+  static constexpr int E = 16 / sizeof(T);
+
+  static __device__ __forceinline__ int shift(const T* row) {
+    return int(reinterpret_cast<uintptr_t>(row) / sizeof(T)) & (E - 1);
+  }
+  // `begin`: the tensor's first element. A piece that starts before it (the
+  // first row's) is filled one element at a time.
+  static __device__ __forceinline__ void fetch(T* to, const T* row, const T* begin, int hidden, int lane, int tpr) {
+    const int d = shift(row), pieces = (d + hidden + E - 1) / E;
+    for (int i = lane; i < pieces; i += tpr) {
+      const T* q = row - d + i * E;
+      if (q >= begin) {
+        const int rest = d + hidden - i * E, bytes = (rest < E ? rest : E) * int(sizeof(T));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         uint32_t(__cvta_generic_to_shared(to + i * E))),
+                     "l"(q), "r"(bytes)
+                     : "memory");
+      } else {
+        for (int e = d; e < E && e < d + hidden; ++e) to[i * E + e] = q[e];
+      }
+    }
+  }
+};
+
+// The way back: a row of B-byte elements that its threads have put into shared
+// memory, at the elements that its place in memory is shifted by. Whole pieces
+// are stored as such (stores of single elements off the boundary leave parts of
+// 32-byte sectors, and took three times as long).
+template <int B>
+struct OutWindow {
+  static constexpr int E = 16 / B;
+  uint8_t* to;     // the row
+  uint8_t* stage;  // the window
+
+  __device__ __forceinline__ int shift() const { return int(reinterpret_cast<uintptr_t>(to) & 15) / B; }
+  __device__ __forceinline__ uint8_t* element(int i) const { return stage + (shift() + i) * B; }
+  __device__ __forceinline__ void flush(int hidden, int lane, int tpr) const {
+    const int d = shift(), pieces = (d + hidden + E - 1) / E;
+    for (int i = lane; i < pieces; i += tpr) {
+      const int first = i * E - d;  // the piece's first element
+      if (first >= 0 && first + E <= hidden) {
+        *reinterpret_cast<uint4*>(to + first * B) = *reinterpret_cast<const uint4*>(stage + i * 16);
+      } else {
+        for (int e = first < 0 ? 0 : first; e < first + E && e < hidden; ++e) {
+          if constexpr (B == 1) to[e] = *element(e);
+          else if constexpr (B == 2)
+            reinterpret_cast<uint16_t*>(to)[e] = *reinterpret_cast<const uint16_t*>(element(e));
+          else
+            reinterpret_cast<uint32_t*>(to)[e] = *reinterpret_cast<const uint32_t*>(element(e));
+        }
+      }
+    }
+  }
+};
+
+// Elements of a row's window, which has room for all that its threads read.
+template <typename T, int K>
+struct Staged {
+  const T* base;  // the row's element 0
+  const Part<K, false>& part;
+
+  __device__ __forceinline__ void get(int k, Pair (&f)[4]) const {
+    const T* p = base + part.at[k];
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float<T>(p[j * 32]);
+    if (part.left[k] <= 7 * 32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j * 32 >= part.left[k]) v[j] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = pair(v[2 * j], v[2 * j + 1]);
+  }
+};
+
+// From the fp32 sum of a row to everything that is stored. part.left is 0 for
+// threads without a row. STAGED: the outputs go through `stage`, whose
+// contents (the sources) every thread has read.
+template <typename T, bool F8, bool VEC, bool STAGED, int K, typename Weight>
+__device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool live,
+                                           const Part<K, VEC>& part,
+                                           const Pair (&h)[K][4], const Weight& wv, float* red, uint32_t* top_red,
+                                           T* stage = nullptr) {
+  const int tpr = a.tpr;
+  Pair sum = pair(0.0f, 0.0f), f[4];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (part.left[k] > 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = fma(h[k][j], h[k][j], sum);
+    }
+  const long long out = row * a.hidden;
+  const OutWindow<int(sizeof(T))> hw{reinterpret_cast<uint8_t*>(static_cast<T*>(a.h) + out),
+                                     reinterpret_cast<uint8_t*>(stage)};
+  const OutWindow<F8 ? 1 : int(sizeof(T))> yw{static_cast<uint8_t*>(a.y) + out * (F8 ? 1 : int(sizeof(T))),
+                                              reinterpret_cast<uint8_t*>(a.h ? stage + a.window : stage)};
+  const auto put_h = [&] {
+    if (a.h) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float e[8];
+        split(h[k], e);
+        T* to = static_cast<T*>(a.h) + out;
+        if constexpr (STAGED) to = reinterpret_cast<T*>(hw.element(0));
+        store8<T, VEC>(to + part.at[k], e, part.kStep, STAGED ? kAll : part.left[k]);
+      }
+    }
+  };
+  if constexpr (!STAGED) put_h();
+  const float s = row_sum(sum_of(sum), tpr, red);
+  const float rstd = rsqrtf(fmaf(s, a.inv_hidden, a.eps));
+  if (live && part.lane == 0) a.rstd[row] = rstd;
+  if constexpr (STAGED) {  // behind every thread's last read of a source
+    if (tpr <= 32) __syncwarp();  // else row_sum has a barrier
+    put_h();
+  }
+  const Pair r2 = pair(rstd, rstd);
+  float y[K][8];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    wv.get(k, f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = h[k][j] * r2 * f[j];
+    split(f, y[k]);
+  }
+  uint8_t* const y0 = STAGED ? yw.element(0) : yw.to;
+  if constexpr (!F8) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      store8<T, VEC>(reinterpret_cast<T*>(y0) + part.at[k], y[k], part.kStep, STAGED ? kAll : part.left[k]);
+  } else {
+    uint32_t most = 0;
+    if (a.group == 0 || a.group > 8 * tpr) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (part.left[k] > 0) most = max(most, top_of<VEC>(y[k], part.kStep, part.left[k]));
+    }
+    float inv[8];
+    if (a.group == 0) {
+      const float scale = scale_of(row_max(most, tpr, top_red));
+      if (live && part.lane == 0) a.scale[row] = scale;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) inv[j] = reciprocal(scale);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (a.group) group_scales<VEC>(a, y[k], most, tpr, row, part.at[k], part.left[k], inv);
+      store_e4m3<VEC>(y0 + part.at[k], y[k], inv, part.kStep, STAGED ? kAll : part.left[k]);
+    }
+  }
+  if constexpr (STAGED) {
+    row_sync(tpr);
+    if (a.h) hw.flush(a.hidden, part.lane, tpr);
+    yw.flush(a.hidden, part.lane, tpr);
   }
 }
 
 // One row per tpr threads, in registers: every load is issued before the
 // first value is used, and a row's threads meet once (twice with one e4m3
-// scale per row). W: the weight's type; MANY: more than one partial sum.
-template <typename T, typename W, bool F8, bool VEC, bool MANY, int K>
-__global__ void __launch_bounds__(max_threads(VEC, MANY)) norm_kernel(const __grid_constant__ FwdArgs a) {
+// scale per row). Octets on their boundary. W: the weight's type; MANY: more
+// than one partial sum.
+template <typename T, typename W, bool F8, bool MANY, int K>
+__global__ void __launch_bounds__(max_threads(MANY)) norm_kernel(const __grid_constant__ FwdArgs a) {
   __shared__ float red[32];
   __shared__ uint32_t top_red[32];
-  const int tpr = a.tpr, hidden = a.hidden;
+  const int tpr = a.tpr;
   const int lane = tpr > 32 ? threadIdx.x : threadIdx.x & (tpr - 1);
   const long long row = tpr > 32 ? (long long)blockIdx.x
                                  : (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
   const bool live = row < a.rows;  // every thread stays for the shuffles
   const Row from(live ? row : 0, a.split);
-  Part<K, VEC> part(lane, tpr, hidden);
+  Part<K, true> part(lane, tpr, a.hidden);
   // Four partial sums at a time, with the first of them the residual too.
   constexpr int N = MANY ? 4 : 1;
-  Load<T, VEC, K> xv[N], rv;
-  Load<W, VEC, K> wv;
+  Load<T, true, K> xv[N], rv;
+  Load<W, true, K> wv;
   Pair h[K][4], f[4];
 #pragma unroll 1
   for (int s0 = 0; s0 < (MANY ? a.parts : 1); s0 += N) {
@@ -275,58 +442,45 @@ __global__ void __launch_bounds__(max_threads(VEC, MANY)) norm_kernel(const __gr
 #pragma unroll
     for (int k = 0; k < K; ++k) part.left[k] = 0;
   }
-  Pair sum = pair(0.0f, 0.0f);
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-    if (part.left[k] > 0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fma(h[k][j], h[k][j], sum);
-    }
-  const long long out = row * a.hidden;
-  if (a.h) {
+  finish_row<T, F8, true, false, K>(a, row, live, part, h, wv, red, top_red);
+}
+
+// The same for rows off the vector boundary, which go through shared memory:
+// all sources of a row are on their way at once without a register held for
+// them, and single elements come out of shared memory. A row has a warp or a block.
+template <typename T, typename W, bool F8, int K>
+__global__ void __launch_bounds__(512) norm_staged_kernel(const __grid_constant__ FwdArgs a) {
+  extern __shared__ uint4 smem[];
+  __shared__ float red[32];
+  __shared__ uint32_t top_red[32];
+  const int tpr = a.tpr, lane = tpr > 32 ? threadIdx.x : threadIdx.x & 31, slot = tpr > 32 ? 0 : threadIdx.x >> 5;
+  const long long row = tpr > 32 ? (long long)blockIdx.x : (long long)blockIdx.x * (blockDim.x >> 5) + slot;
+  if (row >= a.rows) return;  // a whole warp
+  const Row from(row, a.split);
+  const int sources = a.parts + (a.residual.p ? 1 : 0);
+  T* const stage = reinterpret_cast<T*>(smem) + slot * a.windows * a.window;
+  for (int s = 0; s < sources; ++s) {
+    const Rows& t = s < a.parts ? a.x[s] : a.residual;
+    Window<T>::fetch(stage + s * a.window, from.of<T>(t), static_cast<const T*>(t.p), a.hidden, lane, tpr);
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  const Part<K, false> part(lane, tpr, a.hidden);
+  Load<W, false, K> wv;
+  wv.load(static_cast<const W*>(a.weight), part);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  row_sync(tpr);
+  Pair h[K][4], f[4];
+  for (int s = 0; s < sources; ++s) {
+    const T* r = from.of<T>(s < a.parts ? a.x[s] : a.residual);
+    const Staged<T, K> v{stage + s * a.window + Window<T>::shift(r), part};
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float e[8];
-      split(h[k], e);
-      store8<T, VEC>(static_cast<T*>(a.h) + out + part.at[k], e, part.step, part.left[k]);
+      v.get(k, f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[k][j] = s ? h[k][j] + f[j] : f[j];
     }
   }
-  const float s = row_sum(sum_of(sum), tpr, red);
-  const float rstd = rsqrtf(fmaf(s, a.inv_hidden, a.eps));
-  if (live && lane == 0) a.rstd[row] = rstd;
-  const Pair r2 = pair(rstd, rstd);
-  float y[K][8];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    wv.get(k, f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = h[k][j] * r2 * f[j];
-    split(f, y[k]);
-  }
-  if constexpr (!F8) {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      store8<T, VEC>(static_cast<T*>(a.y) + out + part.at[k], y[k], part.step, part.left[k]);
-  } else {
-    uint32_t most = 0;
-    if (a.group == 0 || a.group > 8 * tpr) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (part.left[k] > 0) most = max(most, top_of<VEC>(y[k], part.step, part.left[k]));
-    }
-    float inv[8];
-    if (a.group == 0) {
-      const float scale = scale_of(row_max(most, tpr, top_red));
-      if (live && lane == 0) a.scale[row] = scale;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) inv[j] = reciprocal(scale);
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (a.group) group_scales<VEC>(a, y[k], most, tpr, row, part.at[k], part.left[k], inv);
-      store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + out + part.at[k], y[k], inv, part.step, part.left[k]);
-    }
-  }
+  finish_row<T, F8, false, true, K>(a, row, true, part, h, wv, red, top_red, stage);
 }
 
 // The sum of every partial and the residual at eight elements.
@@ -397,7 +551,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_co
       float y[8];
       sum8<T, VEC>(a, from, part, h);
       normal(part, rstd, h, y);
-      top = max(top, top_of<VEC>(y, part.step, part.left[0]));
+      top = max(top, top_of<VEC>(y, part.kStep, part.left[0]));
     });
     const float scale = scale_of(row_max(top, kLongThreads, top_red));
     if (threadIdx.x == 0) a.scale[row] = scale;
@@ -412,23 +566,23 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_co
       sum8<T, VEC>(a, from, part, h);
       normal(part, rstd, h, y);
       split(h, e);
-      if (a.h) store8<T, VEC>(static_cast<T*>(a.h) + out + at, e, part.step, left);
+      if (a.h) store8<T, VEC>(static_cast<T*>(a.h) + out + at, e, part.kStep, left);
     }
     if constexpr (F8) {
       if (a.group) group_scales<VEC>(a, y, 0, kLongThreads, row, at, left, inv);
-      store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + out + at, y, inv, part.step, left);
+      store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + out + at, y, inv, part.kStep, left);
     } else {
-      store8<T, VEC>(static_cast<T*>(a.y) + out + at, y, part.step, left);
+      store8<T, VEC>(static_cast<T*>(a.y) + out + at, y, part.kStep, left);
     }
   });
 }
 
 // A row of the gradient, from this thread's elements: adds to dw's part and
-// stores dx.
-template <typename T, typename W, bool VEC, int K, typename In>
-__device__ __forceinline__ void finish_grad(const BwdArgs& a, long long row, bool live, const Part<K, VEC>& part,
+// stores the row of dx.
+template <typename T, typename W, bool VEC, bool STAGED, int K, typename In>
+__device__ __forceinline__ void finish_grad(const BwdArgs& a, bool live, const Part<K, VEC>& part,
                                             const In& dy, const In& h, const In& dh, float rstd,
-                                            const Load<W, VEC, K>& wv, Pair (&acc)[K][4], float* red) {
+                                            const Load<W, VEC, K>& wv, Pair (&acc)[K][4], float* red, T* dx) {
   Pair g[K][4], n[K][4], sum = pair(0.0f, 0.0f);
   const Pair r2 = pair(rstd, rstd);
 #pragma unroll
@@ -460,7 +614,7 @@ __device__ __forceinline__ void finish_grad(const BwdArgs& a, long long row, boo
     }
     float f[8];
     split(e, f);
-    store8<T, VEC>(static_cast<T*>(a.dx) + row * a.hidden + part.at[k], f, part.step, live ? part.left[k] : 0);
+    store8<T, VEC>(dx + part.at[k], f, part.kStep, STAGED ? kAll : live ? part.left[k] : 0);
   }
 }
 
@@ -470,6 +624,7 @@ template <int K, bool VEC>
 __device__ __forceinline__ void store_partial(const BwdArgs& a, const Part<K, VEC>& part, const Pair (&acc)[K][4],
                                               float* slots) {
   const int tpr = a.tpr;
+  op_nearly_done();
   float* to = a.partial + (long long)blockIdx.x * a.hidden;
   if (tpr <= 32) to = slots + (threadIdx.x / tpr) * a.hidden;
 #pragma unroll
@@ -478,7 +633,7 @@ __device__ __forceinline__ void store_partial(const BwdArgs& a, const Part<K, VE
     split(acc[k], f);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j * part.step < part.left[k]) to[part.at[k] + j * part.step] = f[j];
+      if (j * part.kStep < part.left[k]) to[part.at[k] + j * part.kStep] = f[j];
   }
   if (tpr <= 32) {
     __syncthreads();
@@ -501,16 +656,16 @@ __device__ __forceinline__ void clear(Pair (&acc)[K][4]) {
 
 // Each block walks over rows and keeps its columns' part of dw in registers;
 // the parts go to `partial` and dw_kernel adds them in block order.
-template <typename T, typename W, bool VEC, int K>
+template <typename T, typename W, int K>
 __global__ void __launch_bounds__(kRingThreads) norm_backward_kernel(const __grid_constant__ BwdArgs a) {
   __shared__ float red[2][32];
   __shared__ float slots[256 * 8 * K];
   const int tpr = a.tpr;
   const int lane = tpr > 32 ? threadIdx.x : threadIdx.x & (tpr - 1);
   const int per = tpr > 32 ? 1 : blockDim.x / tpr, slot = tpr > 32 ? 0 : threadIdx.x / tpr;
-  const Part<K, VEC> part(lane, tpr, a.hidden);
+  const Part<K, true> part(lane, tpr, a.hidden);
   Pair acc[K][4];
-  Load<W, VEC, K> wv;
+  Load<W, true, K> wv;
   wv.load(static_cast<const W*>(a.weight), part);
   clear<K>(acc);
   const long long stride = (long long)gridDim.x * per;
@@ -519,13 +674,14 @@ __global__ void __launch_bounds__(kRingThreads) norm_backward_kernel(const __gri
     const bool live = row < a.rows;
     const long long r = live ? row : a.rows - 1;
     const Row from(r, a.split);
-    Load<T, VEC, K> dy, h, dh;
+    Load<T, true, K> dy, h, dh;
     dy.load(from.of<T>(a.dy), part);
     h.load(from.of<T>(a.h), part);
     if (a.dh.p) dh.load(from.of<T>(a.dh), part);
-    finish_grad<T, W, VEC, K>(a, row, live, part, dy, h, dh, a.rstd[r], wv, acc, red[turn & 1]);
+    finish_grad<T, W, true, false, K>(a, live, part, dy, h, dh, a.rstd[r], wv, acc, red[turn & 1],
+                                static_cast<T*>(a.dx) + row * a.hidden);
   }
-  store_partial<K, VEC>(a, part, acc, slots);
+  store_partial<K, true>(a, part, acc, slots);
 }
 
 // A thread's own ring in shared memory: kStages rows of its octets of a 16-bit
@@ -602,13 +758,76 @@ __global__ void __launch_bounds__(kRingThreads) norm_backward_ring_kernel(const 
       ring.read(s, 0, dy);
       ring.read(s, 1, h);
       if (a.dh.p) ring.read(s, 2, dh);
-      finish_grad<T, W, true, K>(a, row, row < a.rows, part, dy, h, dh, rstds[s], wv, acc, red[s & 1]);
+      finish_grad<T, W, true, false, K>(a, row < a.rows, part, dy, h, dh, rstds[s], wv, acc, red[s & 1],
+                                    static_cast<T*>(a.dx) + row * a.hidden);
       row += stride;
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   store_partial<K, true>(a, part, acc, reinterpret_cast<float*>(smem));
+}
+
+// The same for rows off the boundary, a warp or a block to each: the rows on
+// their way are windows that the row's threads share, so they meet between a
+// stage's copies and its use, and between its use and the next copies. dx has
+// a window of its own.
+constexpr int kStagesOff = 3;
+
+template <typename T, typename W, int K>
+__global__ void __launch_bounds__(kStagedThreads) norm_backward_staged_kernel(const __grid_constant__ BwdArgs a) {
+  extern __shared__ uint4 smem[];
+  __shared__ float red[2][32];
+  const int tpr = a.tpr, lane = tpr > 32 ? threadIdx.x : threadIdx.x & 31;
+  const int per = tpr > 32 ? 1 : blockDim.x >> 5, slot = tpr > 32 ? 0 : threadIdx.x >> 5;
+  const Part<K, false> part(lane, tpr, a.hidden);
+  const int sources = a.dh.p ? 3 : 2;
+  T* const ring = reinterpret_cast<T*>(smem) + slot * (kStagesOff * sources + 1) * a.window;
+  const long long first = (long long)blockIdx.x * per + slot, stride = (long long)gridDim.x * per;
+  long long ahead = first;
+  const auto fetch = [&](int stage) {
+    if (ahead < a.rows) {
+      const Row from(ahead, a.split);
+      T* to = ring + stage * sources * a.window;
+      const auto one = [&](const Rows& t) {
+        Window<T>::fetch(to, from.of<T>(t), static_cast<const T*>(t.p), a.hidden, lane, tpr);
+        to += a.window;
+      };
+      one(a.dy);
+      one(a.h);
+      if (a.dh.p) one(a.dh);
+    }
+    ahead += stride;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kStagesOff - 1; ++s) fetch(s);
+  Pair acc[K][4];
+  Load<W, false, K> wv;
+  wv.load(static_cast<const W*>(a.weight), part);
+  clear<K>(acc);
+  int stage = 0, turn = 0;
+  for (long long row = first; row < a.rows; row += stride, ++turn) {
+    const float rstd = a.rstd[row];
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStagesOff - 2) : "memory");
+    row_sync(tpr);
+    fetch(stage == 0 ? kStagesOff - 1 : stage - 1);  // the stage of the row before
+    const Row from(row, a.split);
+    const T* at = ring + stage * sources * a.window;
+    const Staged<T, K> dy{at + Window<T>::shift(from.of<T>(a.dy)), part},
+        h{at + a.window + Window<T>::shift(from.of<T>(a.h)), part},
+        dh{at + 2 * a.window + Window<T>::shift(from.of<T>(a.dh)), part};
+    const OutWindow<int(sizeof(T))> out{reinterpret_cast<uint8_t*>(static_cast<T*>(a.dx) + row * a.hidden),
+                                        reinterpret_cast<uint8_t*>(ring + kStagesOff * sources * a.window)};
+    finish_grad<T, W, false, true, K>(a, true, part, dy, h, dh, rstd, wv, acc, red[turn & 1],
+                                      reinterpret_cast<T*>(out.element(0)));
+    row_sync(tpr);
+    out.flush(a.hidden, lane, tpr);  // read before the row's threads meet again
+    stage = stage == kStagesOff - 1 ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  store_partial<K, false>(a, part, acc, reinterpret_cast<float*>(smem));
 }
 
 // Long rows: dx with two passes over the row (the second from L2) ...
@@ -657,7 +876,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_backward_long_kernel(const 
     for (int j = 0; j < 4; ++j) e[j] = fma(fma(n[j], pair(c, c), g[j]), r2, e[j]);
     float f[8];
     split(e, f);
-    store8<T, VEC>(static_cast<T*>(a.dx) + row * a.hidden + part.at[0], f, part.step, part.left[0]);
+    store8<T, VEC>(static_cast<T*>(a.dx) + row * a.hidden + part.at[0], f, part.kStep, part.left[0]);
   });
 }
 
@@ -686,7 +905,7 @@ __global__ void __launch_bounds__(256) dw_long_kernel(const __grid_constant__ Bw
   split(acc, f);
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (j * part.step < part.left[0]) to[j * part.step] = f[j];
+    if (j * part.kStep < part.left[0]) to[j * part.kStep] = f[j];
 }
 
 // dw[col] = sum of the blocks' parts: a warp-wide strip of 32 columns per
@@ -696,8 +915,11 @@ __global__ void __launch_bounds__(1024) dw_kernel(const float* partial, int part
   __shared__ float sum[32][33];
   const int col = blockIdx.x * 32 + threadIdx.x;
   float s = 0.0f;
-  if (col < hidden)
+  op_wait_for_previous();
+  if (col < hidden) {
+#pragma unroll 8
     for (int p = threadIdx.y; p < parts; p += 32) s += partial[(long long)p * hidden + col];
+  }
   sum[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   s = sum[threadIdx.x][threadIdx.y];  // transposed: a warp adds one column
@@ -714,7 +936,7 @@ constexpr int kRingSmem = 220 * 1024;  // of an SM's shared memory, for the ring
 // How rows are spread over threads and blocks.
 struct Shape {
   int tpr = 0, threads = 0, k = 0;  // k 0: the long variant
-  bool ring = false;
+  bool ring = false, staged = false;
   size_t smem = 0;
   long long blocks = 0;
 };
@@ -727,48 +949,69 @@ int pow2_at_least(int n) {
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// `k` octets a thread; rows that take up to 32 threads share a block (and a warp).
-void spread(Shape& s, int octets, int k) {
+
+// `k` octets a thread; rows of up to 32 threads share a block: `warp` gives each a whole warp.
+void spread(Shape& s, int octets, int k, bool warp) {
   s.k = k;
   if (octets <= 32 * k) {
-    s.tpr = pow2_at_least(int(ceil_div(octets, k)));
+    s.tpr = warp ? 32 : pow2_at_least(int(ceil_div(octets, k)));
     s.threads = 256;
   } else {
     s.tpr = s.threads = int(ceil_div(ceil_div(octets, 32), k)) * 32;
   }
 }
 
-long long blocks_of(const Shape& s, long long rows) {
-  return s.tpr > 32 ? rows : ceil_div(rows, s.threads / s.tpr);
-}
+int rows_per_block(const Shape& s) { return s.tpr > 32 ? 1 : s.threads / s.tpr; }
 
-Shape shape_fwd(long long rows, int hidden, int most, int sms) {
+// Elements from one staged row to the next: room for every thread's elements, and a piece more for its shift.
+int window_of(const Shape& s, int es) { return s.tpr * 8 * s.k + 16 / es; }
+
+// Aligned rows stay in registers; others go through shared memory, `windows`
+// (sources or outputs) of them for each row, where two blocks fit an SM. What
+// is too long for either is read again in each pass.
+Shape shape_fwd(long long rows, int hidden, int es, int windows, bool vec, bool many, int sms) {
   Shape s;
-  const int octets = int(ceil_div(hidden, 8));
+  const int octets = int(ceil_div(hidden, 8)), most = vec ? max_threads(many) : 512;
   s.blocks = rows;
   if (octets > 2 * most) return s;
-  int k = octets > most || rows > sms ? 2 : 1;
-  spread(s, octets, k);
-  s.blocks = blocks_of(s, rows);
+  spread(s, octets, octets > most || (vec ? rows > sms : octets > 32) ? 2 : 1, !vec);
+  s.blocks = ceil_div(rows, rows_per_block(s));
+  if (!vec) {
+    s.staged = true;
+    s.smem = size_t(rows_per_block(s)) * size_t(windows) * size_t(window_of(s, es)) * size_t(es);
+    if (s.smem > size_t(kRingSmem) / 2) {
+      s = Shape{};
+      s.blocks = rows;
+    }
+  }
   return s;
 }
 
-Shape shape_bwd(long long rows, int hidden, int es, int sms) {
+Shape shape_bwd(long long rows, int hidden, int es, bool vec, int sms) {
   Shape s;
   const int octets = int(ceil_div(hidden, 8));
-  if (octets > 2 * kRingThreads) {  // blocks that share dw's columns
+  bool fits = octets <= 2 * kRingThreads;
+  if (fits) {
+    spread(s, octets, 2, !vec);
+    // Sized for three sources, so that the parts of dw do not depend on them.
+    s.smem = vec ? size_t(kStages) * 3u * 2u * size_t(s.threads) * 16u
+                 : size_t(rows_per_block(s)) * (kStagesOff * 3u + 1u) * size_t(window_of(s, es)) * size_t(es);
+    const bool room = s.smem <= size_t(kRingSmem);
+    s.ring = vec && es == 2 && room;
+    s.staged = !vec;
+    fits = vec || room;
+  }
+  if (!fits) {  // blocks that share dw's columns
+    s = Shape{};
     const long long columns = ceil_div(octets, 256), splits = ceil_div(8ll * sms, columns);
     s.blocks = splits < rows ? splits : rows;
     return s;
   }
-  spread(s, octets, 2);
-  // Sized for three sources, so that the parts of dw do not depend on them.
-  s.smem = size_t(kStages) * 3u * 2u * size_t(s.threads) * 16u;
-  const int by_threads = kRingThreads / s.threads, by_smem = int(size_t(kRingSmem) / s.smem);
-  s.ring = es == 2 && by_smem > 0;
-  // As many blocks as are resident, but with four rows each before every SM has more than one.
-  const long long fit = (long long)sms * (s.ring && by_smem < by_threads ? by_smem : by_threads);
-  const long long most = blocks_of(s, rows), few = ceil_div(most, 4);
+  const int by_threads = (vec ? kRingThreads : kStagedThreads) / s.threads;
+  const int by_smem = s.ring || s.staged ? int(size_t(kRingSmem) / s.smem) : by_threads;
+  // As many as are resident, but with four rows each before every SM has more than one.
+  const long long fit = (long long)sms * (by_smem < by_threads ? by_smem : by_threads);
+  const long long most = ceil_div(rows, rows_per_block(s)), few = ceil_div(most, 4);
   s.blocks = most < sms ? most : few < sms ? sms : few < fit ? few : fit;
   return s;
 }
@@ -782,28 +1025,29 @@ RowSplit split_by(long long inner) {
   return s;
 }
 
-template <typename T, typename W, bool F8, bool VEC>
-const void* fwd_kernel(int k, bool many) {
-  if (k == 1) return many ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, VEC, true, 1>)
-                          : reinterpret_cast<const void*>(norm_kernel<T, W, F8, VEC, false, 1>);
-  if (k == 2) return many ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, VEC, true, 2>)
-                          : reinterpret_cast<const void*>(norm_kernel<T, W, F8, VEC, false, 2>);
-  return reinterpret_cast<const void*>(norm_long_kernel<T, W, F8, VEC>);
+template <typename T, typename W, bool F8>
+const void* fwd_kernel(bool vec, bool many, const Shape& s) {
+  if (s.staged) return s.k == 1 ? reinterpret_cast<const void*>(norm_staged_kernel<T, W, F8, 1>)
+                                : reinterpret_cast<const void*>(norm_staged_kernel<T, W, F8, 2>);
+  if (s.k == 1) return many ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, true, 1>)
+                            : reinterpret_cast<const void*>(norm_kernel<T, W, F8, false, 1>);
+  if (s.k == 2) return many ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, true, 2>)
+                            : reinterpret_cast<const void*>(norm_kernel<T, W, F8, false, 2>);
+  return vec ? reinterpret_cast<const void*>(norm_long_kernel<T, W, F8, true>)
+             : reinterpret_cast<const void*>(norm_long_kernel<T, W, F8, false>);
 }
 
 // The kernels of an input and a weight type.
 template <typename T, typename W>
 struct Kernels {
-  static const void* fwd(bool f8, bool vec, int k, bool many) {
-    if (f8) return vec ? fwd_kernel<T, W, true, true>(k, many) : fwd_kernel<T, W, true, false>(k, many);
-    return vec ? fwd_kernel<T, W, false, true>(k, many) : fwd_kernel<T, W, false, false>(k, many);
+  static const void* fwd(bool f8, bool vec, bool many, const Shape& s) {
+    return f8 ? fwd_kernel<T, W, true>(vec, many, s) : fwd_kernel<T, W, false>(vec, many, s);
   }
   static const void* bwd(bool vec, const Shape& s) {
     if constexpr (sizeof(T) == 2)
-      if (s.k && vec && s.ring) return reinterpret_cast<const void*>(norm_backward_ring_kernel<T, W, 2>);
-    if (s.k)
-      return vec ? reinterpret_cast<const void*>(norm_backward_kernel<T, W, true, 2>)
-                 : reinterpret_cast<const void*>(norm_backward_kernel<T, W, false, 2>);
+      if (s.ring) return reinterpret_cast<const void*>(norm_backward_ring_kernel<T, W, 2>);
+    if (s.staged) return reinterpret_cast<const void*>(norm_backward_staged_kernel<T, W, 2>);
+    if (s.k) return reinterpret_cast<const void*>(norm_backward_kernel<T, W, 2>);
     return vec ? reinterpret_cast<const void*>(norm_backward_long_kernel<T, W, true>)
                : reinterpret_cast<const void*>(norm_backward_long_kernel<T, W, false>);
   }
@@ -818,9 +1062,9 @@ const void* by_types(int dtype, bool wf32, F f) {
   }
 }
 
-cudaError_t launch(const void* fn, const Shape& s, bool ring, unsigned blocks, void** argv, cudaStream_t stream) {
+cudaError_t launch(const void* fn, const Shape& s, unsigned blocks, void** argv, cudaStream_t stream) {
   size_t smem = 0;
-  if (ring) {
+  if (s.ring || s.staged) {
     smem = s.smem;
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return e;
@@ -905,7 +1149,9 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   k.residual = {a->residual, a->r_outer, a->r_inner};
   if (a->residual) vec = vec && octets_fit(a->residual, a->r_outer, a->r_inner, es);
   vec = vec && octets_fit(a->y, 0, 0, f8 ? 1 : es) && (!a->h || octets_fit(a->h, 0, 0, es));
-  const Shape s = shape_fwd(a->rows, a->hidden, max_threads(vec, a->parts > 1), dev.sms());
+  const int sources = a->parts + (a->residual ? 1 : 0), outputs = a->h ? 2 : 1;
+  k.windows = sources > outputs ? sources : outputs;
+  const Shape s = shape_fwd(a->rows, a->hidden, es, k.windows, vec, a->parts > 1, dev.sms());
   k.weight = a->weight;
   k.y = a->y;
   k.scale = a->scale;
@@ -918,12 +1164,13 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   k.group = a->group;
   k.groups = a->group ? (a->hidden + a->group - 1) / a->group : 1;
   k.tpr = s.tpr;
+  k.window = window_of(s, es);
   k.eps = a->eps;
   k.inv_hidden = 1.0f / float(a->hidden);
   const void* fn = by_types(a->dtype, a->weight_dtype == NB_NORM_FLOAT32,
-                            [&](auto kernels) { return kernels.fwd(f8, vec, s.k, a->parts > 1); });
+                            [&](auto kernels) { return kernels.fwd(f8, vec, a->parts > 1, s); });
   void* argv[] = {&k};
-  const cudaError_t e = launch(fn, s, false, unsigned(s.blocks), argv, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch(fn, s, unsigned(s.blocks), argv, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : op_refuse(err, errcap, "launch of the norm failed", int(e));
 }
 
@@ -931,7 +1178,9 @@ extern "C" uint64_t nb_add_rms_norm_backward_workspace(int device, int64_t rows,
   const int es = size_of(dtype);
   OpDevice dev(device);
   if (dev.error() || rows < 0 || hidden < 1 || !es) return 0;
-  return uint64_t(shape_bwd(rows, hidden, es, dev.sms()).blocks) * uint64_t(hidden) * sizeof(float);
+  const long long on = shape_bwd(rows, hidden, es, true, dev.sms()).blocks;
+  const long long off = shape_bwd(rows, hidden, es, false, dev.sms()).blocks;
+  return uint64_t(on > off ? on : off) * uint64_t(hidden) * sizeof(float);
 }
 
 extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, char* err, size_t errcap) {
@@ -946,7 +1195,10 @@ extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, c
     return op_refuse(err, errcap, "bad arguments: null or misaligned tensor");
   OpDevice dev(a->device);
   if (dev.error()) return op_refuse(err, errcap, "cannot use the device", int(dev.error()));
-  const Shape s = shape_bwd(a->rows, a->hidden, es, dev.sms());
+  const bool vec = a->hidden % 8 == 0 && octets_fit(a->weight, 0, 0, ws) &&
+                   octets_fit(a->dy, a->dy_outer, a->dy_inner, es) && octets_fit(a->h, a->h_outer, a->h_inner, es) &&
+                   (!a->dh || octets_fit(a->dh, a->dh_outer, a->dh_inner, es)) && octets_fit(a->dx, 0, 0, es);
+  const Shape s = shape_bwd(a->rows, a->hidden, es, vec, dev.sms());
   const long long parts = s.blocks;
   if (a->rows && (misplaced(a->workspace, 4) || a->workspace_bytes < uint64_t(parts) * uint64_t(a->hidden) * 4))
     return op_refuse(err, errcap, "bad arguments: the workspace is too small");
@@ -965,17 +1217,15 @@ extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, c
   k.split = split_by(a->inner);
   k.hidden = a->hidden;
   k.tpr = s.tpr;
+  k.window = window_of(s, es);
   k.inv_hidden = 1.0f / float(a->hidden);
-  const bool vec = a->hidden % 8 == 0 && octets_fit(a->weight, 0, 0, ws) &&
-                   octets_fit(a->dy, a->dy_outer, a->dy_inner, es) && octets_fit(a->h, a->h_outer, a->h_inner, es) &&
-                   (!a->dh || octets_fit(a->dh, a->dh_outer, a->dh_inner, es)) && octets_fit(a->dx, 0, 0, es);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   void* argv[] = {&k};
   cudaError_t e = cudaSuccess;
   if (a->rows) {
     const void* fn = by_types(a->dtype, a->weight_dtype == NB_NORM_FLOAT32,
                               [&](auto kernels) { return kernels.bwd(vec, s); });
-    e = launch(fn, s, s.ring && vec, unsigned(s.k ? parts : a->rows), argv, st);
+    e = launch(fn, s, unsigned(s.k ? parts : a->rows), argv, st);
     if (e == cudaSuccess && !s.k) {
       fn = a->dtype == NB_NORM_FLOAT32   ? pick_dw_long<float>(vec)
            : a->dtype == NB_NORM_FLOAT16 ? pick_dw_long<__half>(vec)
@@ -992,7 +1242,7 @@ extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, c
     int count = int(parts), hidden = a->hidden;
     void* dw = a->dweight;
     void* dargv[] = {&partial, &count, &hidden, &dw};
-    e = cudaLaunchKernel(fn, dim3(unsigned((hidden + 31) / 32)), dim3(32, 32), dargv, 0, st);
+    e = op_launch_after(fn, dim3(unsigned((hidden + 31) / 32)), dim3(32, 32), dargv, st);
   }
   return e == cudaSuccess ? 0 : op_refuse(err, errcap, "launch of the norm's gradient failed", int(e));
 }

@@ -65,13 +65,14 @@ def test_norm_refuses_overlapping_outputs():
 
 def test_row_strides():
     a = torch.empty(6, 5, 64)
-    assert norm._rows([(a, "a")]) == (1, [(64, 0)])
-    assert norm._rows([(a[:, :3], "a")]) == (3, [(320, 64)])
-    assert norm._rows([(a[:, 1], "a")]) == (1, [(320, 0)])
-    assert norm._rows([(a[:, :3], "a"), (torch.empty(6, 3, 64), "b")]) == (3, [(320, 64), (192, 64)])
-    assert norm._rows([(a[:, :, :32], "a")]) == (1, [(64, 0)])
-    assert norm._rows([(a[:1, :1], "a")]) == (1, [(64, 0)])
-    assert norm._rows([(torch.empty(64).expand(6, 5, 64), "a")]) == (1, [(0, 0)])
+    assert norm._rows([a]) == (1, [64], [0])
+    assert norm._rows([a[:, :3]]) == (3, [320], [64])
+    assert norm._rows([a[:, 1]]) == (1, [320], [0])
+    assert norm._rows([a[:, :3], torch.empty(6, 3, 64)]) == (3, [320, 192], [64, 64])
+    assert norm._rows([torch.empty(6, 3, 64), a[:, :3]]) == (3, [192, 320], [64, 64])
+    assert norm._rows([a[:, :, :32]]) == (1, [64], [0])
+    assert norm._rows([a[:1, :1]]) == (1, [64], [0])
+    assert norm._rows([torch.empty(64).expand(6, 5, 64)]) == (1, [0], [0])
 
 
 f = torch.zeros
@@ -139,7 +140,7 @@ def test_c_entry_points_refuse_with_a_message():
     a = 1 << 20  # an aligned address that no refused call touches
 
     def fwd(x0=a, parts=1, y=a, rows=4, inner=1, hidden=64, dtype=9, wdtype=9, odtype=9, group=0, eps=1e-6, w=a):
-        p = norm._FWD.pack(x0, *[a] * 7, *[hidden] * 8, *[0] * 8, 0, 0, 0, w, y, a, a, a, rows, inner, 0, hidden,
+        p = norm._FWD[8].pack(x0, *[a] * 7, *[hidden] * 8, *[0] * 8, 0, 0, 0, w, y, a, a, a, rows, inner, 0, hidden,
                            parts, dtype, wdtype, odtype, group, eps)
         return L.nb_add_rms_norm(p, None, err, 256), err.value
 
