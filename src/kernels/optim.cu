@@ -133,10 +133,10 @@ __device__ __forceinline__ uint32_t signs4(float a, float b, float c, float d) {
 
 // Where a lane's eight elements are: neighbours, or 32 apart so that single
 // elements coalesce. Both cover the warp's 256.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, unsigned long long warp_base, int lane, long long left, bool vec,
+template <bool VEC, typename T>
+__device__ __forceinline__ void load8(const T* p, unsigned long long warp_base, int lane, long long left,
                                       float (&f)[8]) {
-  if (vec) {
+  if constexpr (VEC) {
     unpack<T>(load_oct(p + warp_base + lane * 8), f);
   } else {
 #pragma unroll
@@ -145,10 +145,10 @@ __device__ __forceinline__ void load8(const T* p, unsigned long long warp_base, 
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, unsigned long long warp_base, int lane, long long left, bool vec,
+template <bool VEC, typename T>
+__device__ __forceinline__ void store8(T* p, unsigned long long warp_base, int lane, long long left,
                                        const float (&f)[8]) {
-  if (vec) {
+  if constexpr (VEC) {
     store_vec<T>(p + warp_base + lane * 8, pack<T>(f));
   } else {
 #pragma unroll
@@ -157,11 +157,12 @@ __device__ __forceinline__ void store8(T* p, unsigned long long warp_base, int l
   }
 }
 
+template <bool VEC>
 __device__ __forceinline__ void load8_e4m3(const void* p, unsigned long long warp_base, int lane, long long left,
-                                           bool vec, float (&f)[8]) {
+                                           float (&f)[8]) {
   const uint8_t* b = static_cast<const uint8_t*>(p) + warp_base;
   uint2 q = make_uint2(0, 0);
-  if (vec) {
+  if constexpr (VEC) {
     q = *reinterpret_cast<const uint2*>(b + lane * 8);
   } else {
 #pragma unroll
@@ -174,10 +175,10 @@ __device__ __forceinline__ void load8_e4m3(const void* p, unsigned long long war
   from_e4m3(q, f);
 }
 
-__device__ __forceinline__ void store8_codes(void* p, unsigned long long warp_base, int lane, long long left, bool vec,
-                                             uint2 q) {
+template <bool VEC>
+__device__ __forceinline__ void store8_codes(void* p, unsigned long long warp_base, int lane, long long left, uint2 q) {
   uint8_t* b = static_cast<uint8_t*>(p) + warp_base;
-  if (vec) {
+  if constexpr (VEC) {
     *reinterpret_cast<uint2*>(b + lane * 8) = q;
   } else {
 #pragma unroll
@@ -186,10 +187,103 @@ __device__ __forceinline__ void store8_codes(void* p, unsigned long long warp_ba
   }
 }
 
+// The step's numbers as the kernel uses them.
+struct StepValues {
+  float scale, lr, size, root;  // size: lr / (1 - b1^t); root: 1 / sqrt(1 - b2^t)
+  unsigned t;
+};
+
+// One warp's 256 elements from `base` on. VEC: all there, and every address
+// on an octet's boundary.
+template <typename P, typename C, typename G, bool S8, bool VEC, typename Args>
+__device__ __forceinline__ void step_tile(const Args& a, const StepValues& r, const Entry& e,
+                                          const unsigned long long* from, unsigned long long base, long long left,
+                                          int lane) {
+  constexpr bool kCopy = sizeof(C) != sizeof(P);
+  float g[8], m[8], v[8], p[8];
+  load8<VEC>(static_cast<const P*>(e.param), base, lane, left, p);
+  float ms = 0.0f, vs = 0.0f;
+  if constexpr (S8) {
+    ms = e.m_scale[base >> 8];
+    vs = e.v_scale[base >> 8];
+    load8_e4m3<VEC>(e.m, base, lane, left, m);
+    load8_e4m3<VEC>(e.v, base, lane, left, v);
+  } else {
+    load8<VEC>(static_cast<const float*>(e.m), base, lane, left, m);
+    load8<VEC>(static_cast<const float*>(e.v), base, lane, left, v);
+  }
+  load8<VEC>(reinterpret_cast<const G*>(from[0]), base, lane, left, g);
+#pragma unroll 1
+  for (int k = 1; k < a.parts; ++k) {
+    float f[8];
+    load8<VEC>(reinterpret_cast<const G*>(from[k]), base, lane, left, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] += f[j];
+  }
+  const float keep = 1.0f - r.lr * e.decay;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const Pair gg = pair(g[j], g[j + 1]) * pair(r.scale, r.scale);
+    Pair mm = pair(m[j], m[j + 1]), vv = pair(v[j], v[j + 1]);
+    if constexpr (S8) {
+      mm = mm * pair(ms, ms);
+      vv = vv * pair(vs, vs);
+      vv = vv * vv;
+    }
+    mm = mm * pair(a.b1, a.b1) + gg * pair(a.b1c, a.b1c);
+    vv = vv * pair(a.b2, a.b2) + gg * gg * pair(a.b2c, a.b2c);
+    split(mm, m[j], m[j + 1]);
+    split(vv, v[j], v[j + 1]);
+    const float r0 = sqrtf(v[j]), r1 = sqrtf(v[j + 1]);
+    float n0, n1, d0, d1, k0, k1;
+    split(mm * pair(r.size, r.size), n0, n1);
+    split(pair(r0, r1) * pair(r.root, r.root) + pair(a.eps, a.eps), d0, d1);
+    split(pair(p[j], p[j + 1]) * pair(keep, keep), k0, k1);
+    // Off by two units in the last place at most, of a term far below p.
+    p[j] = k0 - __fdividef(n0, d0);
+    p[j + 1] = k1 - __fdividef(n1, d1);
+    if constexpr (S8) {
+      v[j] = r0;
+      v[j + 1] = r1;
+    }
+  }
+  store8<VEC>(static_cast<P*>(e.param), base, lane, left, p);
+  if constexpr (kCopy) store8<VEC>(static_cast<C*>(e.copy), base, lane, left, p);
+  if constexpr (!S8) {
+    store8<VEC>(static_cast<float*>(e.m), base, lane, left, m);
+    store8<VEC>(static_cast<float*>(e.v), base, lane, left, v);
+  } else {
+    ms = scale_of(__reduce_max_sync(~0u, top_of(m)));
+    vs = scale_of(__reduce_max_sync(~0u, top_of(v)));
+    const float mi = 1.0f / ms, vi = 1.0f / vs;
+    const uint32_t key = a.seed + r.t * 0x165667B1u + e.index * 0x3C6EF35Fu + uint32_t(base >> 32) * 0x6A09E667u;
+    uint32_t at = (uint32_t(base) + (VEC ? lane * 8 : lane)) * 0x9E3779B9u + key;
+    const uint32_t next = VEC ? 0x9E3779B9u : 32u * 0x9E3779B9u;
+    uint32_t mw[8], vw[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bits = mix(at);
+      at += next;
+      mw[j] = round_random(m[j] * mi, __byte_perm(bits, 0, 0x4324));  // the upper half
+      // A positive root has the least code at least, which is 2^-9.
+      const float y = v[j] * vi;
+      vw[j] = round_random(v[j] > 0.0f ? fmaxf(y, 0x1p-9f) : y, __byte_perm(bits, 0, 0x4104));  // the lower half
+    }
+    store8_codes<VEC>(e.m, base, lane, left,
+                 make_uint2(codes4(mw[0], mw[1], mw[2], mw[3]) | signs4(m[0], m[1], m[2], m[3]),
+                            codes4(mw[4], mw[5], mw[6], mw[7]) | signs4(m[4], m[5], m[6], m[7])));
+    store8_codes<VEC>(e.v, base, lane, left,
+                 make_uint2(codes4(vw[0], vw[1], vw[2], vw[3]), codes4(vw[4], vw[5], vw[6], vw[7])));
+    if (lane == 0) {
+      e.m_scale[base >> 8] = ms;
+      e.v_scale[base >> 8] = vs;
+    }
+  }
+}
+
 // P: parameters; C: their copy (P itself: none); G: gradients; S8: states in e4m3.
 template <typename P, typename C, typename G, bool S8, int WORDS>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ AdamArgs<WORDS> a) {
-  constexpr bool kCopy = sizeof(C) != sizeof(P);
+__global__ void __launch_bounds__(kThreads, S8 ? 4 : 3) adamw_kernel(const __grid_constant__ AdamArgs<WORDS> a) {
   float scale = a.s.scale_host;
   if (a.s.scale) scale *= *a.s.scale;
   if (!(fabsf(scale) <= 3.4028235e38f)) return;  // no step
@@ -207,6 +301,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     }
     size = lr * inv1;
   }
+  const StepValues r{scale, lr, size, root, t};
   const Entry* entries = reinterpret_cast<const Entry*>(a.words);
   const unsigned long long* grads = a.words + (size_t)a.count * kEntryWords;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -217,86 +312,9 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     const unsigned long long base = (unsigned long long)(c - e.first) * kChunk + (unsigned)warp * 256u;
     if (base >= e.size) continue;  // the whole warp
     const long long left = (long long)(e.size - base);
-    const bool vec = e.vec && left >= 256;
-    float g[8], m[8], v[8], p[8];
-    load8<P>(static_cast<const P*>(e.param), base, lane, left, vec, p);
-    float ms = 0.0f, vs = 0.0f;
-    if constexpr (S8) {
-      ms = e.m_scale[base >> 8];
-      vs = e.v_scale[base >> 8];
-      load8_e4m3(e.m, base, lane, left, vec, m);
-      load8_e4m3(e.v, base, lane, left, vec, v);
-    } else {
-      load8<float>(static_cast<const float*>(e.m), base, lane, left, vec, m);
-      load8<float>(static_cast<const float*>(e.v), base, lane, left, vec, v);
-    }
-    load8<G>(reinterpret_cast<const G*>(grads[(size_t)i * a.parts]), base, lane, left, vec, g);
-#pragma unroll 1
-    for (int k = 1; k < a.parts; ++k) {
-      float f[8];
-      load8<G>(reinterpret_cast<const G*>(grads[(size_t)i * a.parts + k]), base, lane, left, vec, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] += f[j];
-    }
-    const float keep = 1.0f - lr * e.decay;
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const Pair gg = pair(g[j], g[j + 1]) * pair(scale, scale);
-      Pair mm = pair(m[j], m[j + 1]), vv = pair(v[j], v[j + 1]);
-      if constexpr (S8) {
-        mm = mm * pair(ms, ms);
-        vv = vv * pair(vs, vs);
-        vv = vv * vv;
-      }
-      mm = mm * pair(a.b1, a.b1) + gg * pair(a.b1c, a.b1c);
-      vv = vv * pair(a.b2, a.b2) + gg * gg * pair(a.b2c, a.b2c);
-      split(mm, m[j], m[j + 1]);
-      split(vv, v[j], v[j + 1]);
-      const float r0 = sqrtf(v[j]), r1 = sqrtf(v[j + 1]);
-      float n0, n1, d0, d1, k0, k1;
-      split(mm * pair(size, size), n0, n1);
-      split(pair(r0, r1) * pair(root, root) + pair(a.eps, a.eps), d0, d1);
-      split(pair(p[j], p[j + 1]) * pair(keep, keep), k0, k1);
-      // Off by two units in the last place at most, of a term far below p.
-      p[j] = k0 - __fdividef(n0, d0);
-      p[j + 1] = k1 - __fdividef(n1, d1);
-      if constexpr (S8) {
-        v[j] = r0;
-        v[j + 1] = r1;
-      }
-    }
-    store8<P>(static_cast<P*>(e.param), base, lane, left, vec, p);
-    if constexpr (kCopy) store8<C>(static_cast<C*>(e.copy), base, lane, left, vec, p);
-    if constexpr (!S8) {
-      store8<float>(static_cast<float*>(e.m), base, lane, left, vec, m);
-      store8<float>(static_cast<float*>(e.v), base, lane, left, vec, v);
-    } else {
-      ms = scale_of(__reduce_max_sync(~0u, top_of(m)));
-      vs = scale_of(__reduce_max_sync(~0u, top_of(v)));
-      const float mi = 1.0f / ms, vi = 1.0f / vs;
-      const uint32_t key = a.seed + t * 0x165667B1u + e.index * 0x3C6EF35Fu + uint32_t(base >> 32) * 0x6A09E667u;
-      uint32_t at = (uint32_t(base) + (vec ? lane * 8 : lane)) * 0x9E3779B9u + key;
-      const uint32_t next = vec ? 0x9E3779B9u : 32u * 0x9E3779B9u;
-      uint32_t mw[8], vw[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t bits = mix(at);
-        at += next;
-        mw[j] = round_random(m[j] * mi, __byte_perm(bits, 0, 0x4324));  // the upper half
-        // A positive root has the least code at least, which is 2^-9.
-        const float y = v[j] * vi;
-        vw[j] = round_random(v[j] > 0.0f ? fmaxf(y, 0x1p-9f) : y, __byte_perm(bits, 0, 0x4104));  // the lower half
-      }
-      store8_codes(e.m, base, lane, left, vec,
-                   make_uint2(codes4(mw[0], mw[1], mw[2], mw[3]) | signs4(m[0], m[1], m[2], m[3]),
-                              codes4(mw[4], mw[5], mw[6], mw[7]) | signs4(m[4], m[5], m[6], m[7])));
-      store8_codes(e.v, base, lane, left, vec,
-                   make_uint2(codes4(vw[0], vw[1], vw[2], vw[3]), codes4(vw[4], vw[5], vw[6], vw[7])));
-      if (lane == 0) {
-        e.m_scale[base >> 8] = ms;
-        e.v_scale[base >> 8] = vs;
-      }
-    }
+    const unsigned long long* from = grads + (size_t)i * a.parts;
+    if (e.vec && left >= 256) step_tile<P, C, G, S8, true>(a, r, e, from, base, left, lane);
+    else step_tile<P, C, G, S8, false>(a, r, e, from, base, left, lane);
   }
 }
 
@@ -486,8 +504,8 @@ struct NormHandle {
 };
 
 template <typename E, typename Fill>
-std::vector<Launch> build_launches(const uint64_t* sizes, int count, int parts, const void* const* grad, int sms,
-                                   unsigned chunk, Fill fill) {
+std::vector<Launch> build_launches(const uint64_t* sizes, int count, int parts, const void* const* grad,
+                                   unsigned most_blocks, unsigned chunk, Fill fill) {
   constexpr int kWords = sizeof(E) / 8;
   std::vector<Launch> out;
   for (const TableLaunch& t : pack_tensors(sizes, size_t(count), kLargeWords / (kWords + parts), chunk)) {
@@ -507,8 +525,7 @@ std::vector<Launch> build_launches(const uint64_t* sizes, int count, int parts, 
             reinterpret_cast<unsigned long long>(grad[size_t(i) * size_t(parts) + size_t(p)]);
     }
     l.large = l.words.size() > size_t(kSmallWords);
-    const unsigned fit = unsigned(sms) * (2048 / kThreads);
-    l.blocks = l.chunks < fit ? l.chunks : fit;
+    l.blocks = l.chunks < most_blocks ? l.chunks : most_blocks;
     out.push_back(std::move(l));
   }
   return out;
@@ -581,7 +598,12 @@ extern "C" void* nb_adamw_create(const nb_adamw_t* a, char* err, size_t errcap) 
     h->seed = a->seed * 0x27D4EB2Fu;
     h->kernel[0] = adamw_for<kSmallWords>(a->param_dtype, a->copy_dtype, a->grad_dtype, s8);
     h->kernel[1] = adamw_for<kLargeWords>(a->param_dtype, a->copy_dtype, a->grad_dtype, s8);
-    h->launches = build_launches<Entry>(a->size, a->count, a->parts, a->grad, dev.sms(), kChunk, [&](int i, Entry& e) {
+    // 32-bit states are bound by HBM, and a block per chunk sweeps it in order
+    // (201 M elements: 834 us, against 870 to 966 with 3 to 24 blocks an SM that
+    // stride over the chunks); 8-bit ones by their arithmetic, so that a block's
+    // setup counts (255 M: 898 us with 12 an SM, 986 with a block per chunk).
+    const unsigned most = s8 ? unsigned(dev.sms()) * 12u : ~0u;
+    h->launches = build_launches<Entry>(a->size, a->count, a->parts, a->grad, most, kChunk, [&](int i, Entry& e) {
       e.param = a->param[i];
       e.copy = cs ? a->copy[i] : nullptr;
       e.m = a->m[i];
@@ -681,7 +703,8 @@ extern "C" void* nb_grad_norm_create(int device, int count, int parts, int dtype
     h->parts = parts;
     h->kernel[0] = grad_norm_for<kSmallWords>(dtype);
     h->kernel[1] = grad_norm_for<kLargeWords>(dtype);
-    h->launches = build_launches<GradEntry>(size, count, parts, grad, dev.sms(), kNormChunk, [&](int i, GradEntry& e) {
+    h->launches = build_launches<GradEntry>(size, count, parts, grad, unsigned(dev.sms()) * 8u, kNormChunk,
+                                             [&](int i, GradEntry& e) {
       bool vec = true;
       for (int p = 0; p < parts; ++p)
         vec = vec && on_boundary(grad[size_t(i) * size_t(parts) + size_t(p)], size_t(gs) * 8);

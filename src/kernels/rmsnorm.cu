@@ -54,7 +54,7 @@ struct FwdArgs {
   float* rstd;
   long long rows;
   RowSplit split;
-  int hidden, parts, group, tpr, groups;
+  int hidden, parts, group, group_log, tpr, groups;
   int window, windows;  // elements between staged rows, and a row's number of them
   float eps, inv_hidden;
 };
@@ -180,7 +180,11 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[8], cons
 
 // 1 / scale, for a scale of at least 2^-126: off by an ulp at most, so that a
 // value within that of the middle between two codes may take either.
-__device__ __forceinline__ float reciprocal(float scale) { return __fdividef(1.0f, scale); }
+__device__ __forceinline__ float reciprocal(float scale) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+  return r;
+}
 
 // The reciprocals of the scales of groups of 32, 64 or 128 columns, one for each
 // of a thread's eight values; the group's first thread stores its scale. `whole`: the
@@ -198,7 +202,7 @@ __device__ __forceinline__ void group_scales(const FwdArgs& a, const float (&y)[
     }
     for (int o = lanes >> 1; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
     const float s = scale_of(top), i = reciprocal(s);
-    if (left > 0 && (at & (a.group - 1)) == 0) to[unsigned(at) / unsigned(a.group)] = s;
+    if (left > 0 && (at & (a.group - 1)) == 0) to[at >> a.group_log] = s;
 #pragma unroll
     for (int j = 0; j < 8; ++j) inv[j] = i;
   } else {  // a group is one, two or four neighbouring j of a warp's lanes
@@ -219,7 +223,7 @@ __device__ __forceinline__ void group_scales(const FwdArgs& a, const float (&y)[
       const float s = scale_of(__reduce_max_sync(~0u, top[j]));
       inv[j] = reciprocal(s);
       const int col = at + j * 32;
-      if (j * 32 < left && (col & (a.group - 1)) == 0) to[unsigned(col) / unsigned(a.group)] = s;
+      if (j * 32 < left && (col & (a.group - 1)) == 0) to[col >> a.group_log] = s;
     }
   }
 }
@@ -1162,6 +1166,7 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   k.hidden = a->hidden;
   k.parts = a->parts;
   k.group = a->group;
+  k.group_log = a->group == 128 ? 7 : a->group == 64 ? 6 : 5;
   k.groups = a->group ? (a->hidden + a->group - 1) / a->group : 1;
   k.tpr = s.tpr;
   k.window = window_of(s, es);
