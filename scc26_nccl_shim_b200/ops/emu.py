@@ -43,11 +43,16 @@ def _stream(t):
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
-def raw_stream(device: int) -> int:
-    """The current stream of `device` as a cudaStream_t."""
+@functools.lru_cache(maxsize=1)
+def _current_raw_stream():
     import torch
     fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # no Stream object is made
-    return fast(device) if fast else torch.cuda.current_stream(device).cuda_stream
+    return fast or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def raw_stream(device: int) -> int:
+    """The current stream of `device` as a cudaStream_t."""
+    return _current_raw_stream()(device)
 
 
 def reduce(srcs, dsts, op="sum", nranks=None, scalars=None, nbytes=None):

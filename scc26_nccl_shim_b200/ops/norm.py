@@ -29,6 +29,7 @@ GROUPS = (0, 32, 64, 128)
 # nb_norm_t, by the number of partial sums (the arrays' other places are zero)
 _FWD = [struct.Struct(f"{n}Q{8 * (8 - n)}x{n}q{8 * (8 - n)}x{n}q{8 * (8 - n)}xQ2q5Q2q7if") for n in range(9)]
 _BWD = struct.Struct("Q2qQ2qQ2qQQQQQQ2q4i")    # nb_norm_grad_t
+_CONTIGUOUS = torch.contiguous_format
 _ERR = 256
 
 
@@ -205,9 +206,9 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
         raise ValueError(f"the tensors must be on a CUDA device, got {dev}")
     device = dev.index
     if out is None:
-        y = _empty(shape, ydtype, dev)
+        y = torch.empty_like(x0, dtype=ydtype, memory_format=_CONTIGUOUS)
         scale = _empty(lead + (groups,), torch.float32, dev) if f8 else None
-        h = _empty(shape, dtype, dev) if sums else x0
+        h = torch.empty_like(x0, memory_format=_CONTIGUOUS) if sums else x0
         rstd = _empty(lead, torch.float32, dev)
     if residual is None:
         r = (0, 0, 0)
@@ -280,8 +281,8 @@ def add_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
     if dev.type != "cuda":
         raise ValueError(f"the tensors must be on a CUDA device, got {dev}")
     device, rows = dev.index, rstd.numel()
-    dx = _empty(shape, dtype, dev)
-    dw = _empty((hidden,), weight.dtype, dev)
+    dx = torch.empty_like(h, memory_format=_CONTIGUOUS)
+    dw = torch.empty_like(weight)
     nbytes = _workspace_bytes(device, rows, hidden, code)
     ws = _empty((nbytes // 4,), torch.float32, dev)
     s = (dh.data_ptr(), outers[2], inners[2]) if dh is not None else (0, 0, 0)

@@ -65,8 +65,9 @@ struct GradEntry {
 };
 constexpr int kGradEntryWords = sizeof(GradEntry) / 8;
 
-// The list's room: few tensors keep the launch's parameters small.
-constexpr int kSmallWords = 448, kLargeWords = 4000;
+// The list's room. A launch with 32 KB of parameters takes about 1 us longer to
+// queue than one with 10 KB, which hold some 120 tensors.
+constexpr int kSmallWords = 1200, kLargeWords = 4000;
 
 struct StepScalars {
   const long long* t;
@@ -88,7 +89,7 @@ struct AdamArgs {
   unsigned long long words[WORDS];
 };
 static_assert(sizeof(AdamArgs<kLargeWords>) <= 32764, "kernel parameters");
-static_assert(sizeof(AdamArgs<kSmallWords>) <= 4096, "kernel parameters");
+
 
 template <int WORDS>
 struct GradArgs {
@@ -193,25 +194,10 @@ struct StepValues {
   unsigned t;
 };
 
-// One warp's 256 elements from `base` on. VEC: all there, and every address
-// on an octet's boundary.
-template <typename P, typename C, typename G, bool S8, bool VEC, typename Args>
-__device__ __forceinline__ void step_tile(const Args& a, const StepValues& r, const Entry& e,
-                                          const unsigned long long* from, unsigned long long base, long long left,
-                                          int lane) {
-  constexpr bool kCopy = sizeof(C) != sizeof(P);
-  float g[8], m[8], v[8], p[8];
-  load8<VEC>(static_cast<const P*>(e.param), base, lane, left, p);
-  float ms = 0.0f, vs = 0.0f;
-  if constexpr (S8) {
-    ms = e.m_scale[base >> 8];
-    vs = e.v_scale[base >> 8];
-    load8_e4m3<VEC>(e.m, base, lane, left, m);
-    load8_e4m3<VEC>(e.v, base, lane, left, v);
-  } else {
-    load8<VEC>(static_cast<const float*>(e.m), base, lane, left, m);
-    load8<VEC>(static_cast<const float*>(e.v), base, lane, left, v);
-  }
+// The sum of the partial gradients, times the scale.
+template <bool VEC, typename G, typename Args>
+__device__ __forceinline__ void load_gradient(const Args& a, const unsigned long long* from, unsigned long long base,
+                                              int lane, long long left, float scale, float (&g)[8]) {
   load8<VEC>(reinterpret_cast<const G*>(from[0]), base, lane, left, g);
 #pragma unroll 1
   for (int k = 1; k < a.parts; ++k) {
@@ -220,64 +206,133 @@ __device__ __forceinline__ void step_tile(const Args& a, const StepValues& r, co
 #pragma unroll
     for (int j = 0; j < 8; ++j) g[j] += f[j];
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) g[j] *= scale;
+}
+
+// a x + b y: the products and their sum are rounded one by one, so that the
+// states do not depend on what a compiler fuses (it fuses paired products and
+// sums even where they are written apart).
+__device__ __forceinline__ void blend(Pair x, float a, Pair y, float b, float& lo, float& hi) {
+  float x0, x1, y0, y1;
+  split(x * pair(a, a), x0, x1);
+  split(y * pair(b, b), y0, y1);
+  lo = __fadd_rn(x0, y0);
+  hi = __fadd_rn(x1, y1);
+}
+
+// One warp's 256 elements from `base` on. VEC: all there, and every address
+// on an octet's boundary. States in fp32.
+template <typename P, typename C, typename G, bool VEC, typename Args>
+__device__ __forceinline__ void step_tile(const Args& a, const StepValues& r, const Entry& e,
+                                          const unsigned long long* from, unsigned long long base, long long left,
+                                          int lane) {
+  float g[8], m[8], v[8], p[8];
+  load8<VEC>(static_cast<const P*>(e.param), base, lane, left, p);
+  load8<VEC>(static_cast<const float*>(e.m), base, lane, left, m);
+  load8<VEC>(static_cast<const float*>(e.v), base, lane, left, v);
+  load_gradient<VEC, G>(a, from, base, lane, left, r.scale, g);
   const float keep = 1.0f - r.lr * e.decay;
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
-    const Pair gg = pair(g[j], g[j + 1]) * pair(r.scale, r.scale);
-    Pair mm = pair(m[j], m[j + 1]), vv = pair(v[j], v[j + 1]);
-    if constexpr (S8) {
-      mm = mm * pair(ms, ms);
-      vv = vv * pair(vs, vs);
-      vv = vv * vv;
-    }
-    mm = mm * pair(a.b1, a.b1) + gg * pair(a.b1c, a.b1c);
-    vv = vv * pair(a.b2, a.b2) + gg * gg * pair(a.b2c, a.b2c);
-    split(mm, m[j], m[j + 1]);
-    split(vv, v[j], v[j + 1]);
-    const float r0 = sqrtf(v[j]), r1 = sqrtf(v[j + 1]);
-    float n0, n1, d0, d1, k0, k1;
-    split(mm * pair(r.size, r.size), n0, n1);
-    split(pair(r0, r1) * pair(r.root, r.root) + pair(a.eps, a.eps), d0, d1);
-    split(pair(p[j], p[j + 1]) * pair(keep, keep), k0, k1);
-    // Off by two units in the last place at most, of a term far below p.
-    p[j] = k0 - __fdividef(n0, d0);
-    p[j + 1] = k1 - __fdividef(n1, d1);
-    if constexpr (S8) {
-      v[j] = r0;
-      v[j + 1] = r1;
-    }
+    const Pair gg = pair(g[j], g[j + 1]);
+    blend(pair(m[j], m[j + 1]), a.b1, gg, a.b1c, m[j], m[j + 1]);
+    blend(pair(v[j], v[j + 1]), a.b2, gg * gg, a.b2c, v[j], v[j + 1]);
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)  // the quotient is off by two units in the last place at most, and far below p
+    p[j] = p[j] * keep - __fdividef(m[j] * r.size, sqrtf(v[j]) * r.root + a.eps);
   store8<VEC>(static_cast<P*>(e.param), base, lane, left, p);
-  if constexpr (kCopy) store8<VEC>(static_cast<C*>(e.copy), base, lane, left, p);
-  if constexpr (!S8) {
-    store8<VEC>(static_cast<float*>(e.m), base, lane, left, m);
-    store8<VEC>(static_cast<float*>(e.v), base, lane, left, v);
+  if constexpr (sizeof(C) != sizeof(P)) store8<VEC>(static_cast<C*>(e.copy), base, lane, left, p);
+  store8<VEC>(static_cast<float*>(e.m), base, lane, left, m);
+  store8<VEC>(static_cast<float*>(e.v), base, lane, left, v);
+}
+
+// sqrt(x) for x = 0 and from 2^-100 to 2^120: one step of Newton's iteration on
+// x y, y = 1 / sqrt(x), with the residual x - s^2 exact by a fused product
+// (Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990). Without a branch, where sqrtf has one an element; it is sqrtf's result but for
+// a few in a million, which are its neighbours.
+__device__ __forceinline__ Pair root_of(float x0, float x1) {
+  const Pair x = pair(x0, x1), y = pair(rsqrtf(fmaxf(x0, 0x1p-100f)), rsqrtf(fmaxf(x1, 0x1p-100f)));
+  const Pair s = x * y, half = y * pair(0.5f, 0.5f), minus = s * pair(-1.0f, -1.0f);
+  return fma(fma(minus, s, x), half, s);
+}
+
+__device__ __forceinline__ float quotient(float n, float d) {  // d a normal number below 2^126
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return n * r;
+}
+
+// The same with states in e4m3. v is kept as 2^64 v and its root as 2^32
+// sqrt(v) while it is computed, which changes no rounding and keeps the
+// smallest ones normal; a block whose v would overflow so takes the plain way.
+template <typename P, typename C, typename G, bool VEC, typename Args>
+__device__ __forceinline__ void step_tile8(const Args& a, const StepValues& r, const Entry& e,
+                                           const unsigned long long* from, unsigned long long base, long long left,
+                                           int lane) {
+  float g[8], m[8], v[8], p[8];
+  load8<VEC>(static_cast<const P*>(e.param), base, lane, left, p);
+  float ms = e.m_scale[base >> 8], vs = e.v_scale[base >> 8];
+  load8_e4m3<VEC>(e.m, base, lane, left, m);
+  load8_e4m3<VEC>(e.v, base, lane, left, v);
+  load_gradient<VEC, G>(a, from, base, lane, left, r.scale, g);
+  const float big = vs * 0x1p32f;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const Pair gg = pair(g[j], g[j + 1]), gb = gg * pair(0x1p32f, 0x1p32f);
+    const Pair q = pair(v[j], v[j + 1]) * pair(big, big);
+    blend(pair(m[j], m[j + 1]) * pair(ms, ms), a.b1, gg, a.b1c, m[j], m[j + 1]);
+    blend(q * q, a.b2, gb * gb, a.b2c, v[j], v[j + 1]);
+  }
+  if (__reduce_max_sync(~0u, top_of(v)) < 0x7b800000u) {  // 2^120
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) split(root_of(v[j], v[j + 1]), v[j], v[j + 1]);
   } else {
-    ms = scale_of(__reduce_max_sync(~0u, top_of(m)));
-    vs = scale_of(__reduce_max_sync(~0u, top_of(v)));
-    const float mi = 1.0f / ms, vi = 1.0f / vs;
-    const uint32_t key = a.seed + r.t * 0x165667B1u + e.index * 0x3C6EF35Fu + uint32_t(base >> 32) * 0x6A09E667u;
-    uint32_t at = (uint32_t(base) + (VEC ? lane * 8 : lane)) * 0x9E3779B9u + key;
-    const uint32_t next = VEC ? 0x9E3779B9u : 32u * 0x9E3779B9u;
-    uint32_t mw[8], vw[8];
+    load8_e4m3<VEC>(e.v, base, lane, left, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t bits = mix(at);
-      at += next;
-      mw[j] = round_random(m[j] * mi, __byte_perm(bits, 0, 0x4324));  // the upper half
-      // A positive root has the least code at least, which is 2^-9.
-      const float y = v[j] * vi;
-      vw[j] = round_random(v[j] > 0.0f ? fmaxf(y, 0x1p-9f) : y, __byte_perm(bits, 0, 0x4104));  // the lower half
+      const float q = v[j] * vs;
+      v[j] = sqrtf(__fadd_rn(q * q * a.b2, g[j] * g[j] * a.b2c)) * 0x1p32f;
     }
-    store8_codes<VEC>(e.m, base, lane, left,
-                 make_uint2(codes4(mw[0], mw[1], mw[2], mw[3]) | signs4(m[0], m[1], m[2], m[3]),
-                            codes4(mw[4], mw[5], mw[6], mw[7]) | signs4(m[4], m[5], m[6], m[7])));
-    store8_codes<VEC>(e.v, base, lane, left,
-                 make_uint2(codes4(vw[0], vw[1], vw[2], vw[3]), codes4(vw[4], vw[5], vw[6], vw[7])));
-    if (lane == 0) {
-      e.m_scale[base >> 8] = ms;
-      e.v_scale[base >> 8] = vs;
-    }
+  }
+  const float keep = 1.0f - r.lr * e.decay, root = r.root * 0x1p-32f;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float n0, n1, d0, d1, k0, k1;
+    split(pair(m[j], m[j + 1]) * pair(r.size, r.size), n0, n1);
+    split(fma(pair(v[j], v[j + 1]), pair(root, root), pair(a.eps, a.eps)), d0, d1);
+    split(pair(p[j], p[j + 1]) * pair(keep, keep), k0, k1);
+    p[j] = k0 - quotient(n0, d0);
+    p[j + 1] = k1 - quotient(n1, d1);
+  }
+  store8<VEC>(static_cast<P*>(e.param), base, lane, left, p);
+  if constexpr (sizeof(C) != sizeof(P)) store8<VEC>(static_cast<C*>(e.copy), base, lane, left, p);
+  ms = scale_of(__reduce_max_sync(~0u, top_of(m)));
+  vs = scale_of(__float_as_uint(__uint_as_float(__reduce_max_sync(~0u, top_of(v))) * 0x1p-32f));
+  const float mi = 1.0f / ms, vi = 1.0f / vs * 0x1p-32f;
+  const uint32_t key = a.seed + r.t * 0x165667B1u + e.index * 0x3C6EF35Fu + uint32_t(base >> 32) * 0x6A09E667u;
+  uint32_t at = (uint32_t(base) + (VEC ? lane * 8 : lane)) * 0x9E3779B9u + key;
+  const uint32_t next = VEC ? 0x9E3779B9u : 32u * 0x9E3779B9u;
+  uint32_t mw[8], vw[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t bits = mix(at);
+    at += next;
+    mw[j] = round_random(m[j] * mi, __byte_perm(bits, 0, 0x4324));  // the upper half
+    // A positive root has the least code at least, which is 2^-9.
+    const float y = v[j] * vi;
+    vw[j] = round_random(v[j] > 0.0f ? fmaxf(y, 0x1p-9f) : y, __byte_perm(bits, 0, 0x4104));  // the lower half
+  }
+  store8_codes<VEC>(e.m, base, lane, left,
+                    make_uint2(codes4(mw[0], mw[1], mw[2], mw[3]) | signs4(m[0], m[1], m[2], m[3]),
+                               codes4(mw[4], mw[5], mw[6], mw[7]) | signs4(m[4], m[5], m[6], m[7])));
+  store8_codes<VEC>(e.v, base, lane, left,
+                    make_uint2(codes4(vw[0], vw[1], vw[2], vw[3]), codes4(vw[4], vw[5], vw[6], vw[7])));
+  if (lane == 0) {
+    e.m_scale[base >> 8] = ms;
+    e.v_scale[base >> 8] = vs;
   }
 }
 
@@ -313,8 +368,14 @@ __global__ void __launch_bounds__(kThreads, S8 ? 4 : 3) adamw_kernel(const __gri
     if (base >= e.size) continue;  // the whole warp
     const long long left = (long long)(e.size - base);
     const unsigned long long* from = grads + (size_t)i * a.parts;
-    if (e.vec && left >= 256) step_tile<P, C, G, S8, true>(a, r, e, from, base, left, lane);
-    else step_tile<P, C, G, S8, false>(a, r, e, from, base, left, lane);
+    const bool vec = e.vec && left >= 256;
+    if constexpr (S8) {
+      if (vec) step_tile8<P, C, G, true>(a, r, e, from, base, left, lane);
+      else step_tile8<P, C, G, false>(a, r, e, from, base, left, lane);
+    } else {
+      if (vec) step_tile<P, C, G, true>(a, r, e, from, base, left, lane);
+      else step_tile<P, C, G, false>(a, r, e, from, base, left, lane);
+    }
   }
 }
 

@@ -200,7 +200,8 @@ __device__ __forceinline__ void group_scales(const FwdArgs& a, const float (&y)[
       lanes = tpr;
       top = whole;
     }
-    for (int o = lanes >> 1; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+    const int in = threadIdx.x & 31;
+    top = __reduce_max_sync(((1u << lanes) - 1u) << (in & ~(lanes - 1)), top);
     const float s = scale_of(top), i = reciprocal(s);
     if (left > 0 && (at & (a.group - 1)) == 0) to[at >> a.group_log] = s;
 #pragma unroll

@@ -261,6 +261,55 @@ def test_8bit_states_follow_the_32bit_ones():
     assert abs(r8.mean() / r32.mean() - 1) < 0.1
 
 
+def test_8bit_roots_are_the_rounded_ones():
+    """The kernel's own square root against torch's rounded one, on a million
+    values over the range that it is used for: with one element a block, the new
+    scale is sqrt(v) times 1/448. It may miss by one unit in the last place
+    where the root lies next to the middle of two numbers: Newton's step leaves
+    an error below 2^-42 of it, so in less than one of 2^17 cases."""
+    m = optim()
+    n = 1 << 20
+    g = torch.Generator(device=DEV).manual_seed(3)
+    scale = torch.exp(torch.rand(n, device=DEV, generator=g) * 60 - 40)  # 4e-18 to 5e8
+    codes = torch.zeros(n * 256, dtype=torch.uint8, device=DEV)
+    codes[::256] = 0x7E  # 448
+    zero = (torch.zeros(n * 256, dtype=torch.uint8, device=DEV).view(E4M3), torch.zeros(n, device=DEV))
+    p, grad = torch.zeros(n * 256, dtype=torch.bfloat16, device=DEV), \
+        torch.zeros(n * 256, dtype=torch.bfloat16, device=DEV)
+    before = scale.clone()
+    opt = m.AdamW([p], [grad], betas=(0.9, 0.7), state="8bit", states=([zero], [(codes.view(E4M3), scale)]))
+    opt.step(5, 0.0)
+    r = before * 448
+    want = torch.sqrt(r * r * 0.7) * torch.tensor(1 / 448, device=DEV)
+    assert ((scale.view(torch.int32) - want.view(torch.int32)).abs() <= 1).all()
+    assert (scale != want).sum() <= n >> 17
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e8, 1e14, 1e18])
+def test_8bit_extreme_gradients(size):
+    """v between the smallest subnormal numbers and the largest ones."""
+    m = optim()
+    p, g = torch.zeros(3000, device=DEV), data(3000, torch.float32, 2, size)
+    opt = m.AdamW([p], [g], betas=BETAS, eps=1e-37, weight_decay=0.0, state="8bit")
+    opt.step(1, LR)
+    v = 0.001 * g.double().square()
+    # In fp32, v below 2^-126 loses bits: off by up to 2^-149 (three roundings).
+    v_tol = 8 * U * v + 3 * 2.0 ** -149
+    low, high = (v - v_tol).clamp(min=0), v + v_tol
+    mhat = g.double()
+    got = -p.double() / LR
+    big = mhat.abs() > 0
+    lo = mhat.abs() / ((high * 1000).sqrt() + 1e-37) * (1 - 64 * U)
+    hi = mhat.abs() / ((low * 1000).sqrt() + 1e-37) * (1 + 64 * U)
+    assert (got.sign() == mhat.sign())[big].all()
+    # (the squares below 2^-149 vanish: the update is then m / eps)
+    assert ((got.abs() >= lo) & (got.abs() <= hi))[big].all()
+    mq, vq = opt.moments(0)
+    assert ((mq.double() - 0.1 * g.double()).abs() <= 0.1 * g.double().abs() / 8 * 1.001 + opt.exp_avg[0][1].double()
+            .repeat_interleave(256)[:3000] * 2.0 ** -9).all()
+    assert vq.isfinite().all()
+
+
 def test_nan_gradient_stays_in_its_block():
     m = optim()
     p, g = data(1024, torch.float32, 1), data(1024, torch.float32, 2)
