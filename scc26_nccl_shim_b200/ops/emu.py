@@ -96,8 +96,9 @@ def bench(kernel: str, n: int, mib: int, dtype: str = "float32", ndst: int = 1, 
           warmup: int = 3) -> dict:
     """Time one kernel on virtual-rank buffers of the current device with CUDA
     events: `reduce` folds n sources of `mib` MiB into ndst destinations;
-    `copy` moves n segments of `mib` MiB. Total sources exceed the 126 MB L2
-    for the default sizes, so every launch streams from HBM."""
+    `copy` moves n segments of `mib` MiB; the norm and optimizer operators take
+    the n sources as their partial ones. Total sources exceed the 126 MB L2 for
+    the default sizes, so every launch streams from HBM."""
     import torch
     dt = getattr(torch, dtype)
     es = torch.tensor([], dtype=dt).element_size()
@@ -111,6 +112,8 @@ def bench(kernel: str, n: int, mib: int, dtype: str = "float32", ndst: int = 1, 
         dsts = [torch.empty_like(s) for s in srcs]
         run = lambda: copy(srcs, dsts, [count * es] * n)  # noqa: E731
         moved = 2 * n * count * es
+    elif kernel in ("norm", "norm_fp8", "norm_backward", "grad_norm", "adamw", "adamw_8bit"):
+        run, moved = _operator(kernel, srcs, torch)
     else:
         raise ValueError(kernel)
     for _ in range(warmup):
@@ -127,11 +130,35 @@ def bench(kernel: str, n: int, mib: int, dtype: str = "float32", ndst: int = 1, 
             "ms": round(ms, 4), "hbm_gbs": round(moved / ms / 1e6, 1)}
 
 
+def _operator(kernel: str, srcs, torch):
+    """One call of a norm or optimizer operator on `srcs` as its partial sums
+    (norm: rows of 4096) or partial gradients, and the bytes it has to move."""
+    from . import norm, optim
+    n, count, es = len(srcs), srcs[0].numel(), srcs[0].element_size()
+    if kernel in ("norm", "norm_fp8", "norm_backward"):
+        xs = [s.view(-1, 4096) for s in srcs]
+        res, w = torch.randn_like(xs[0]), torch.ones(4096, device="cuda", dtype=xs[0].dtype)
+        if kernel == "norm_backward":
+            rstd = torch.ones(xs[0].shape[0], device="cuda")
+            return (lambda: norm.add_rms_norm_backward(xs[0], xs[-1], w, rstd, res)), 4 * count * es
+        fp8 = kernel == "norm_fp8"
+        out = {"out_dtype": norm.E4M3, "group": 128} if fp8 else {}
+        return (lambda: norm.add_rms_norm(xs, w, res, **out)), count * ((n + 2) * es + (1 if fp8 else es))
+    if kernel == "grad_norm":
+        f = optim.GradNorm([srcs])
+        return (lambda: f(1.0)), n * count * es
+    eight = kernel == "adamw_8bit"
+    p = torch.zeros(count, device="cuda")
+    opt = optim.AdamW([p], [srcs], state="8bit" if eight else "float32")
+    return (lambda: opt.step(1, 1e-6)), count * (n * es + 8 + (4 if eight else 16))
+
+
 if __name__ == "__main__":
     import argparse
     import json
-    p = argparse.ArgumentParser(description="time one sm_100a collective kernel on one GPU")
-    p.add_argument("--kernel", choices=["reduce", "copy"], default="reduce")
+    p = argparse.ArgumentParser(description="time one sm_100a kernel on one GPU")
+    p.add_argument("--kernel", choices=["reduce", "copy", "norm", "norm_fp8", "norm_backward", "grad_norm", "adamw",
+                                        "adamw_8bit"], default="reduce")
     p.add_argument("--n", type=int, default=8)
     p.add_argument("--mib", type=int, default=64)
     p.add_argument("--dtype", default="float32")
