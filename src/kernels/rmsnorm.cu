@@ -583,11 +583,11 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_co
 }
 
 // A row of the gradient, from this thread's elements: adds to dw's part and
-// stores the row of dx.
-template <typename T, typename W, bool VEC, bool STAGED, int K, typename In>
+// stores the row of dx. `total`: the sum over the row's threads.
+template <typename T, typename W, bool VEC, bool STAGED, int K, typename In, typename Total>
 __device__ __forceinline__ void finish_grad(const BwdArgs& a, bool live, const Part<K, VEC>& part,
                                             const In& dy, const In& h, const In& dh, float rstd,
-                                            const Load<W, VEC, K>& wv, Pair (&acc)[K][4], float* red, T* dx) {
+                                            const Load<W, VEC, K>& wv, Pair (&acc)[K][4], T* dx, Total total) {
   Pair g[K][4], n[K][4], sum = pair(0.0f, 0.0f);
   const Pair r2 = pair(rstd, rstd);
 #pragma unroll
@@ -606,7 +606,7 @@ __device__ __forceinline__ void finish_grad(const BwdArgs& a, bool live, const P
       }
     }
   }
-  const float c = row_sum(sum_of(sum), a.tpr, red) * -a.inv_hidden;
+  const float c = total(sum_of(sum)) * -a.inv_hidden;
   const Pair c2 = pair(c, c);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -627,10 +627,10 @@ __device__ __forceinline__ void finish_grad(const BwdArgs& a, bool live, const P
 // its slots are added in order.
 template <int K, bool VEC>
 __device__ __forceinline__ void store_partial(const BwdArgs& a, const Part<K, VEC>& part, const Pair (&acc)[K][4],
-                                              float* slots) {
+                                              float* slots, float* to) {
   const int tpr = a.tpr;
   op_nearly_done();
-  float* to = a.partial + (long long)blockIdx.x * a.hidden;
+  float* const block = to;
   if (tpr <= 32) to = slots + (threadIdx.x / tpr) * a.hidden;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -646,7 +646,7 @@ __device__ __forceinline__ void store_partial(const BwdArgs& a, const Part<K, VE
     for (int col = threadIdx.x; col < a.hidden; col += blockDim.x) {
       float s = 0.0f;
       for (int q = 0; q < per; ++q) s += slots[q * a.hidden + col];
-      a.partial[(long long)blockIdx.x * a.hidden + col] = s;
+      block[col] = s;
     }
   }
 }
@@ -683,19 +683,18 @@ __global__ void __launch_bounds__(kRingThreads) norm_backward_kernel(const __gri
     dy.load(from.of<T>(a.dy), part);
     h.load(from.of<T>(a.h), part);
     if (a.dh.p) dh.load(from.of<T>(a.dh), part);
-    finish_grad<T, W, true, false, K>(a, live, part, dy, h, dh, a.rstd[r], wv, acc, red[turn & 1],
-                                static_cast<T*>(a.dx) + row * a.hidden);
+    finish_grad<T, W, true, false, K>(a, live, part, dy, h, dh, a.rstd[r], wv, acc,
+                                      static_cast<T*>(a.dx) + row * a.hidden,
+                                      [&](float s) { return row_sum(s, tpr, red[turn & 1]); });
   }
-  store_partial<K, true>(a, part, acc, slots);
+  store_partial<K, true>(a, part, acc, slots, a.partial + (long long)blockIdx.x * a.hidden);
 }
 
-// A thread's own ring in shared memory: kStages rows of its octets of a 16-bit
+// A thread's own ring in shared memory: a few rows of its octets of a 16-bit
 // type, brought by 16-byte asynchronous copies. Only the thread itself reads
 // them, so a stage needs no barrier: the thread waits for its own copies.
 // Copies of later rows are in flight while a row is reduced, without a
 // register held for them.
-constexpr int kStages = 4;
-
 template <typename T, int K>
 struct Ring {
   uint4* base;
@@ -719,58 +718,87 @@ struct Ring {
   }
 };
 
+// The sum of a value of each of the two blocks of a cluster, the same in
+// both: each stores its own where the other reads it. `box`: two floats of
+// shared memory, used in turn, so that one is read while the other is written.
+__device__ __forceinline__ float pair_sum(float s, float* box, unsigned rank, int turn) {
+  if (threadIdx.x == 0) {
+    uint32_t far;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;"
+        : "=r"(far)
+        : "r"(uint32_t(__cvta_generic_to_shared(box + (turn & 1)))), "r"(rank ^ 1u));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(far), "f"(s) : "memory");
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const float other = *reinterpret_cast<volatile float*>(box + (turn & 1));
+  return rank ? other + s : s + other;
+}
+
 // The same with the next rows on their way (octets on their boundary). A
 // thread without an octet or a row reads what the ring happens to hold and
-// drops it.
-template <typename T, typename W, int K>
+// drops it. PAIR: a row is shared by the two blocks of a cluster, half of the
+// octets each, because one block's registers do not hold it.
+template <typename T, typename W, bool PAIR, int K, int STAGES>
 __global__ void __launch_bounds__(kRingThreads) norm_backward_ring_kernel(const __grid_constant__ BwdArgs a) {
   extern __shared__ uint4 smem[];
   __shared__ float red[2][32];
+  __shared__ float box[2];
   const int tpr = a.tpr;
   const int lane = tpr > 32 ? threadIdx.x : threadIdx.x & (tpr - 1);
   const int per = tpr > 32 ? 1 : blockDim.x / tpr, slot = tpr > 32 ? 0 : threadIdx.x / tpr;
-  const Part<K, true> part(lane, tpr, a.hidden);
+  const unsigned rank = PAIR ? blockIdx.x & 1 : 0;
+  const long long block = PAIR ? blockIdx.x >> 1 : blockIdx.x, blocks = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int half = (a.hidden / 8 + 1) / 2 * 8, from_col = rank * half;
+  const int columns = !PAIR ? a.hidden : rank ? a.hidden - half : half;
+  const Part<K, true> part(lane, tpr, columns);
   const Ring<T, K> ring{smem, a.dh.p ? 3 : 2};
-  const long long stride = (long long)gridDim.x * per;
-  long long ahead = (long long)blockIdx.x * per + slot;
-  float rstds[kStages];  // of the rows on their way
+  const long long stride = blocks * per;
+  long long ahead = block * per + slot;
+  float rstds[STAGES];  // of the rows on their way
   const auto fetch = [&](int stage, float& rstd) {
     rstd = 0.0f;
     if (ahead < a.rows) {
       const Row from(ahead, a.split);
-      ring.fetch(stage, 0, from.of<T>(a.dy), part);
-      ring.fetch(stage, 1, from.of<T>(a.h), part);
-      if (a.dh.p) ring.fetch(stage, 2, from.of<T>(a.dh), part);
+      ring.fetch(stage, 0, from.of<T>(a.dy) + from_col, part);
+      ring.fetch(stage, 1, from.of<T>(a.h) + from_col, part);
+      if (a.dh.p) ring.fetch(stage, 2, from.of<T>(a.dh) + from_col, part);
       rstd = a.rstd[ahead];
     }
     ahead += stride;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) fetch(s, rstds[s]);
+  for (int s = 0; s < STAGES - 1; ++s) fetch(s, rstds[s]);
   Pair acc[K][4];
   Load<W, true, K> wv;
-  wv.load(static_cast<const W*>(a.weight), part);
+  wv.load(static_cast<const W*>(a.weight) + from_col, part);
   clear<K>(acc);
-  for (long long row = (long long)blockIdx.x * per + slot; row - slot < a.rows;) {
+  if constexpr (PAIR)  // both blocks have started before either stores into the other
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  int turn = 0;
+  for (long long row = block * per + slot; row - slot < a.rows;) {
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) {  // the stage is a constant, so rstds stays in registers
+    for (int s = 0; s < STAGES; ++s) {  // the stage is a constant, so rstds stays in registers
       if (row - slot >= a.rows) break;
       // Into the stage of the row before, whose values this thread has used.
-      fetch((s + kStages - 1) % kStages, rstds[(s + kStages - 1) % kStages]);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      fetch((s + STAGES - 1) % STAGES, rstds[(s + STAGES - 1) % STAGES]);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       Load<T, true, K> dy, h, dh;
       ring.read(s, 0, dy);
       ring.read(s, 1, h);
       if (a.dh.p) ring.read(s, 2, dh);
-      finish_grad<T, W, true, false, K>(a, row < a.rows, part, dy, h, dh, rstds[s], wv, acc, red[s & 1],
-                                    static_cast<T*>(a.dx) + row * a.hidden);
+      finish_grad<T, W, true, false, K>(a, row < a.rows, part, dy, h, dh, rstds[s], wv, acc,
+                                        static_cast<T*>(a.dx) + row * a.hidden + from_col, [&](float v) {
+                                          v = row_sum(v, tpr, red[turn & 1]);
+                                          return PAIR ? pair_sum(v, box, rank, turn) : v;
+                                        });
       row += stride;
+      ++turn;
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  store_partial<K, true>(a, part, acc, reinterpret_cast<float*>(smem));
+  store_partial<K, true>(a, part, acc, reinterpret_cast<float*>(smem), a.partial + block * a.hidden + from_col);
 }
 
 // The same for rows off the boundary, a warp or a block to each: the rows on
@@ -824,15 +852,16 @@ __global__ void __launch_bounds__(kStagedThreads) norm_backward_staged_kernel(co
         dh{at + 2 * a.window + Window<T>::shift(from.of<T>(a.dh)), part};
     const OutWindow<int(sizeof(T))> out{reinterpret_cast<uint8_t*>(static_cast<T*>(a.dx) + row * a.hidden),
                                         reinterpret_cast<uint8_t*>(ring + kStagesOff * sources * a.window)};
-    finish_grad<T, W, false, true, K>(a, true, part, dy, h, dh, rstd, wv, acc, red[turn & 1],
-                                      reinterpret_cast<T*>(out.element(0)));
+    finish_grad<T, W, false, true, K>(a, true, part, dy, h, dh, rstd, wv, acc, reinterpret_cast<T*>(out.element(0)),
+                                      [&](float s) { return row_sum(s, tpr, red[turn & 1]); });
     row_sync(tpr);
     out.flush(a.hidden, lane, tpr);  // read before the row's threads meet again
     stage = stage == kStagesOff - 1 ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  store_partial<K, false>(a, part, acc, reinterpret_cast<float*>(smem));
+  store_partial<K, false>(a, part, acc, reinterpret_cast<float*>(smem),
+                          a.partial + (long long)blockIdx.x * a.hidden);
 }
 
 // Long rows: dx with two passes over the row (the second from L2) ...
@@ -936,12 +965,13 @@ __global__ void __launch_bounds__(1024) dw_kernel(const float* partial, int part
 
 // ---------------------------------------------------------------- host
 
+constexpr int kStages = 4;  // rows of a ring
 constexpr int kRingSmem = 220 * 1024;  // of an SM's shared memory, for the rings of its blocks
 
 // How rows are spread over threads and blocks.
 struct Shape {
   int tpr = 0, threads = 0, k = 0;  // k 0: the long variant
-  bool ring = false, staged = false;
+  bool ring = false, staged = false, pair = false;
   size_t smem = 0;
   long long blocks = 0;
 };
@@ -995,9 +1025,10 @@ Shape shape_fwd(long long rows, int hidden, int es, int windows, bool vec, bool 
 Shape shape_bwd(long long rows, int hidden, int es, bool vec, int sms) {
   Shape s;
   const int octets = int(ceil_div(hidden, 8));
-  bool fits = octets <= 2 * kRingThreads;
+  s.pair = vec && es == 2 && octets > 2 * kRingThreads && octets <= 4 * kRingThreads;
+  bool fits = s.pair || octets <= 2 * kRingThreads;
   if (fits) {
-    spread(s, octets, 2, !vec);
+    spread(s, s.pair ? (octets + 1) / 2 : octets, 2, !vec);
     // Sized for three sources, so that the parts of dw do not depend on them.
     s.smem = vec ? size_t(kStages) * 3u * 2u * size_t(s.threads) * 16u
                  : size_t(rows_per_block(s)) * (kStagesOff * 3u + 1u) * size_t(window_of(s, es)) * size_t(es);
@@ -1014,10 +1045,12 @@ Shape shape_bwd(long long rows, int hidden, int es, bool vec, int sms) {
   }
   const int by_threads = (vec ? kRingThreads : kStagedThreads) / s.threads;
   const int by_smem = s.ring || s.staged ? int(size_t(kRingSmem) / s.smem) : by_threads;
-  // As many as are resident, but with four rows each before every SM has more than one.
-  const long long fit = (long long)sms * (by_smem < by_threads ? by_smem : by_threads);
+  // As many as are resident, but with four rows each before every SM has more
+  // than one; of a pair's blocks, half as many.
+  const int places = s.pair ? sms / 2 > 0 ? sms / 2 : 1 : sms;
+  const long long fit = (long long)places * (by_smem < by_threads ? by_smem : by_threads);
   const long long most = ceil_div(rows, rows_per_block(s)), few = ceil_div(most, 4);
-  s.blocks = most < sms ? most : few < sms ? sms : few < fit ? few : fit;
+  s.blocks = most < places ? most : few < places ? places : few < fit ? few : fit;
   return s;
 }
 
@@ -1050,7 +1083,8 @@ struct Kernels {
   }
   static const void* bwd(bool vec, const Shape& s) {
     if constexpr (sizeof(T) == 2)
-      if (s.ring) return reinterpret_cast<const void*>(norm_backward_ring_kernel<T, W, 2>);
+      if (s.ring) return s.pair ? reinterpret_cast<const void*>(norm_backward_ring_kernel<T, W, true, 2, kStages>)
+                                : reinterpret_cast<const void*>(norm_backward_ring_kernel<T, W, false, 2, kStages>);
     if (s.staged) return reinterpret_cast<const void*>(norm_backward_staged_kernel<T, W, 2>);
     if (s.k) return reinterpret_cast<const void*>(norm_backward_kernel<T, W, 2>);
     return vec ? reinterpret_cast<const void*>(norm_backward_long_kernel<T, W, true>)
@@ -1074,7 +1108,20 @@ cudaError_t launch(const void* fn, const Shape& s, unsigned blocks, void** argv,
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return e;
   }
-  return cudaLaunchKernel(fn, dim3(blocks), dim3(unsigned(s.k ? s.threads : kLongThreads)), argv, smem, stream);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  cfg.gridDim = dim3(s.pair ? 2 * blocks : blocks);
+  cfg.blockDim = dim3(unsigned(s.k ? s.threads : kLongThreads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  if (s.pair) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelExC(&cfg, fn, argv);
 }
 
 template <typename T>

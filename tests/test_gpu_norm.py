@@ -107,7 +107,7 @@ def test_partials(parts, residual, dtype):
 
 # Many rows: blocks that walk over them, at each row width's number of threads.
 MANY = [(40000, 8), (30001, 24), (20001, 128), (9000, 256), (5003, 264), (3001, 1024), (2500, 2048), (1300, 4096),
-        (700, 5120), (1000, 8192), (650, 16384)]
+        (700, 5120), (1000, 8192), (400, 8200), (333, 12288), (650, 16384), (150, 16392)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -250,6 +250,19 @@ def test_in_place_and_guards(hidden):
                 assert torch.equal(x2, x)
             if inplace != "residual":
                 assert torch.equal(r2, res)
+
+
+@pytest.mark.parametrize("hidden", [96, 301, 1001, 4096, 5001, 20000])
+def test_one_source_with_a_copy_of_it(hidden):
+    """A single x without a residual, and `h` asked for apart from it."""
+    m = norm()
+    x, w = data((70, hidden), torch.bfloat16, 1), data((hidden,), torch.bfloat16, 2)
+    want = m.add_rms_norm(x, w)
+    out = m.NormOut(torch.empty_like(x), None, torch.full_like(x, 7), torch.empty(70, device=DEV))
+    got = m.add_rms_norm(x, w, out=out)
+    assert torch.equal(got.h, x) and torch.equal(got.y, want.y) and torch.equal(got.rstd, want.rstd)
+    same = m.add_rms_norm(x, w, out=m.NormOut(torch.empty_like(x), None, x, torch.empty(70, device=DEV)))
+    assert same.h is x and torch.equal(same.y, want.y)
 
 
 # ------------------------------------------------------------------ gradient
