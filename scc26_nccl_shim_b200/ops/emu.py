@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import threading
 
 from .. import LIB_PATH, real_nccl_path, require
 from .._core import ALGO, DTYPE, KIND, OP
@@ -41,6 +42,17 @@ def _ptrs(ts):
 def _stream(t):
     import torch
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+class _Err(threading.local):
+    """A buffer for the message of a refused call, one per thread."""
+    size = 256
+
+    def __init__(self):
+        self.buf = C.create_string_buffer(self.size)
+
+
+ERR = _Err()
 
 
 @functools.lru_cache(maxsize=1)

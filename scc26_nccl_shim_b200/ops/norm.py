@@ -30,7 +30,7 @@ GROUPS = (0, 32, 64, 128)
 _FWD = [struct.Struct(f"{n}Q{8 * (8 - n)}x{n}q{8 * (8 - n)}x{n}q{8 * (8 - n)}xQ2q5Q2q7if") for n in range(9)]
 _BWD = struct.Struct("Q2qQ2qQ2qQQQQQQ2q4i")    # nb_norm_grad_t
 _CONTIGUOUS = torch.contiguous_format
-_ERR = 256
+_ERR = emu.ERR.size
 
 
 class NormOut(NamedTuple):
@@ -52,11 +52,6 @@ def lib() -> C.CDLL:
     L.nb_add_rms_norm_backward_workspace.argtypes = [C.c_int, C.c_int64, C.c_int, C.c_int]
     L.nb_add_rms_norm_backward_workspace.restype = C.c_uint64
     return L
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(device: int, rows: int, hidden: int, dtype: int) -> int:
-    return int(lib().nb_add_rms_norm_backward_workspace(device, rows, hidden, dtype))
 
 
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:
@@ -150,6 +145,66 @@ def _empty(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tens
     return torch.empty(shape, dtype=dtype, device=device)
 
 
+class _Plan(NamedTuple):
+    """What a call needs to know of its tensors' types, shapes, strides and
+    devices: made, with all checks of them, once for each combination."""
+    pack: object
+    strides: tuple  # of the inputs, as the struct has them
+    extra: tuple    # of the residual (or dh)
+    tail: tuple     # the struct's numbers
+    device: int
+    ydtype: torch.dtype | None = None
+    scale_shape: tuple | None = None
+    lead: tuple = ()
+    nbytes: int = 0
+
+
+def _describe(t: torch.Tensor) -> tuple:
+    return t.dtype, t.shape, t.stride(), t.device
+
+
+_plans: dict[tuple, _Plan] = {}
+
+
+def _keep(key: tuple, plan: _Plan) -> _Plan:
+    if len(_plans) >= 1024:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _plan_forward(xs: list, weight: torch.Tensor, residual: torch.Tensor | None, eps: float,
+                  out_dtype: torch.dtype | None, group: int) -> _Plan:
+    n = len(xs)
+    if not 1 <= n <= 8:
+        raise ValueError(f"1 to 8 partial sums, got {n}")
+    x0 = xs[0]
+    dtype, shape, dev = x0.dtype, x0.shape, x0.device
+    if dtype not in DTYPE:
+        raise TypeError(f"x: expected fp16, bf16 or fp32, got {dtype}")
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"x: expected shape [..., hidden] with hidden >= 1, got {tuple(shape)}")
+    hidden, lead = shape[-1], tuple(shape[:-1])
+    for i in range(1, n):
+        _like(xs[i], x0, f"x[{i}]")
+    if residual is not None:
+        _like(residual, x0, "residual")
+    wcode = _check_weight(weight, hidden, dtype, dev)
+    f8 = out_dtype == E4M3
+    if not f8 and out_dtype is not None and out_dtype != dtype:
+        raise TypeError(f"out_dtype: expected {dtype} or {E4M3}, got {out_dtype}")
+    if group not in GROUPS or (group and not f8):
+        raise ValueError(f"group: one of {GROUPS} with e4m3 output, else 0, got {group}")
+    if not 0 < eps < math.inf:
+        raise ValueError(f"eps: must be positive, got {eps}")
+    inner, outers, inners = _rows(xs if residual is None else xs + [residual])
+    device = dev.index if dev.type == "cuda" else -1
+    return _Plan(_FWD[n].pack, (*outers[:n], *inners[:n]), (outers[n], inners[n]) if residual is not None else (0, 0),
+                 (math.prod(lead), inner, device, hidden, n, DTYPE[dtype], wcode, NCCL_E4M3 if f8 else DTYPE[dtype],
+                  group, eps), device, E4M3 if f8 else dtype,
+                 lead + (-(-hidden // group) if group else 1,) if f8 else None, lead)
+
+
 def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6,
                  out_dtype: torch.dtype | None = None, group: int = 0, out: NormOut | None = None) -> NormOut:
     """h = x_0 + ... + x_{n-1} + residual; y = h / sqrt(mean(h^2) + eps) * weight.
@@ -171,73 +226,47 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
     x_0 itself, nothing else may overlap).
     """
     xs = [x] if isinstance(x, torch.Tensor) else list(x)
-    n = len(xs)
-    if not 1 <= n <= 8:
-        raise ValueError(f"1 to 8 partial sums, got {n}")
+    key = (eps, out_dtype, group, _describe(weight), None if residual is None else _describe(residual),
+           *[_describe(t) for t in xs])
+    plan = _plans.get(key) or _keep(key, _plan_forward(xs, weight, residual, eps, out_dtype, group))
     x0 = xs[0]
-    dtype, shape, dev = x0.dtype, x0.shape, x0.device
-    code = DTYPE.get(dtype)
-    if code is None:
-        raise TypeError(f"x: expected fp16, bf16 or fp32, got {dtype}")
-    if not shape or shape[-1] < 1:
-        raise ValueError(f"x: expected shape [..., hidden] with hidden >= 1, got {tuple(shape)}")
-    hidden, lead = shape[-1], shape[:-1]
-    sources = xs if residual is None else xs + [residual]
-    for t in sources[1:]:
-        if t.dtype != dtype or t.shape != shape or t.device != dev:
-            _like(t, x0, "residual" if t is residual else "x")
-    wcode = _check_weight(weight, hidden, dtype, dev)
-    if out_dtype is None or out_dtype == dtype:
-        f8, ydtype, ycode = False, dtype, code
-    elif out_dtype == E4M3:
-        f8, ydtype, ycode = True, E4M3, NCCL_E4M3
-    else:
-        raise TypeError(f"out_dtype: expected {dtype} or {E4M3}, got {out_dtype}")
-    if group not in GROUPS or (group and not f8):
-        raise ValueError(f"group: one of {GROUPS} with e4m3 output, else 0, got {group}")
-    if not 0 < eps < math.inf:
-        raise ValueError(f"eps: must be positive, got {eps}")
-    inner, outers, inners = _rows(sources)
-    sums = len(sources) > 1
-    groups = -(-hidden // group) if group else 1
+    alone = residual is None and len(xs) == 1
     if out is not None:
-        y, scale, h, rstd = _check_out(out, xs, weight, residual, ydtype, lead + (groups,) if f8 else None)
-    if dev.type != "cuda":
-        raise ValueError(f"the tensors must be on a CUDA device, got {dev}")
-    device = dev.index
+        _check_out(out, xs, weight, residual, plan)
+    if plan.device < 0:
+        raise ValueError(f"the tensors must be on a CUDA device, got {x0.device}")
     if out is None:
-        y = torch.empty_like(x0, dtype=ydtype, memory_format=_CONTIGUOUS)
-        scale = _empty(lead + (groups,), torch.float32, dev) if f8 else None
-        h = torch.empty_like(x0, memory_format=_CONTIGUOUS) if sums else x0
-        rstd = _empty(lead, torch.float32, dev)
-    if residual is None:
-        r = (0, 0, 0)
+        y = torch.empty_like(x0, dtype=plan.ydtype, memory_format=_CONTIGUOUS)
+        scale = _empty(plan.scale_shape, torch.float32, x0.device) if plan.scale_shape else None
+        h = x0 if alone else torch.empty_like(x0, memory_format=_CONTIGUOUS)
+        rstd = _empty(plan.lead, torch.float32, x0.device)
     else:
-        r = (residual.data_ptr(), outers[n], inners[n])
-    err = C.create_string_buffer(_ERR)
+        y, scale, h, rstd = out
+        if alone and h.data_ptr() == x0.data_ptr():
+            h = x0
+    err = emu.ERR.buf
     rc = lib().nb_add_rms_norm(
-        _FWD[n].pack(*[t.data_ptr() for t in xs], *outers[:n], *inners[:n], *r, weight.data_ptr(), y.data_ptr(),
-                     scale.data_ptr() if f8 else 0, h.data_ptr() if sums or h is not x0 else 0, rstd.data_ptr(),
-                     rstd.numel(), inner, device, hidden, n, code, wcode, ycode, group, eps),
-        emu.raw_stream(device), err, _ERR)
+        plan.pack(*[t.data_ptr() for t in xs], *plan.strides, 0 if residual is None else residual.data_ptr(),
+                  *plan.extra, weight.data_ptr(), y.data_ptr(), 0 if scale is None else scale.data_ptr(),
+                  0 if alone and h is x0 else h.data_ptr(), rstd.data_ptr(), *plan.tail),
+        emu.raw_stream(plan.device), err, _ERR)
     if rc:
         _raise(err, rc)
     return NormOut(y, scale, h, rstd)
 
 
-def _check_out(out, xs, weight, residual, ydtype, scale_shape):
+def _check_out(out: NormOut, xs: list, weight: torch.Tensor, residual: torch.Tensor | None, plan: _Plan) -> None:
     x0 = xs[0]
     inputs = xs + [weight] + ([residual] if residual is not None else [])
-    want = [("y", out.y, x0.shape, ydtype), ("h", out.h, x0.shape, x0.dtype),
+    want = [("y", out.y, x0.shape, plan.ydtype), ("h", out.h, x0.shape, x0.dtype),
             ("rstd", out.rstd, x0.shape[:-1], torch.float32)]
-    if scale_shape is not None:
-        want.append(("scale", out.scale, scale_shape, torch.float32))
+    if plan.scale_shape is not None:
+        want.append(("scale", out.scale, plan.scale_shape, torch.float32))
     elif out.scale is not None:
         raise ValueError("out.scale: only an e4m3 output has scales")
     for name, t, shape, dtype in want:
         if t is None or t.shape != shape or t.dtype != dtype or t.device != x0.device:
             raise ValueError(f"out.{name}: expected {tuple(shape)} of {dtype} on {x0.device}")
-    alone = len(xs) == 1 and residual is None
     for i, (name, t, _, _) in enumerate(want):
         same = [s for s in (xs[0], residual) if name == "h" and s is not None and
                 s.data_ptr() == t.data_ptr() and s.stride() == t.stride()]
@@ -246,9 +275,32 @@ def _check_out(out, xs, weight, residual, ydtype, scale_shape):
         for other in inputs + [w[1] for w in want[i + 1:]]:
             if not any(other is s for s in same) and not _disjoint(t, other):
                 raise ValueError(f"out.{name}: overlaps another tensor of the call")
-    if alone and out.h.data_ptr() == x0.data_ptr():
-        return out.y, out.scale, x0, out.rstd
-    return out.y, out.scale, out.h, out.rstd
+
+
+def _plan_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                   dh: torch.Tensor | None) -> _Plan:
+    dtype, shape, dev = h.dtype, h.shape, h.device
+    if dtype not in DTYPE:
+        raise TypeError(f"h: expected fp16, bf16 or fp32, got {dtype}")
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"h: expected shape [..., hidden] with hidden >= 1, got {tuple(shape)}")
+    hidden = shape[-1]
+    _like(dy, h, "dy")
+    if dh is not None:
+        _like(dh, h, "dh")
+    wcode = _check_weight(weight, hidden, dtype, dev)
+    if rstd.dtype != torch.float32 or rstd.shape != shape[:-1] or not rstd.is_contiguous():
+        raise ValueError(f"rstd: expected {tuple(shape[:-1])} of torch.float32, contiguous")
+    if rstd.device != dev:
+        raise ValueError(f"rstd: on {rstd.device}, expected {dev}")
+    inner, outers, inners = _rows([dy, h] if dh is None else [dy, h, dh])
+    if dev.type != "cuda":
+        raise ValueError(f"the tensors must be on a CUDA device, got {dev}")
+    rows, code = rstd.numel(), DTYPE[dtype]
+    nbytes = int(lib().nb_add_rms_norm_backward_workspace(dev.index, rows, hidden, code))
+    return _Plan(_BWD.pack, ((outers[0], inners[0]), (outers[1], inners[1])),
+                 (0, 0) if dh is None else (outers[2], inners[2]), (rows, inner, dev.index, hidden, code, wcode),
+                 dev.index, nbytes=nbytes)
 
 
 def add_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
@@ -261,37 +313,18 @@ def add_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
     rows of dy * n, in the weight's type, added in an order that depends on
     the sizes alone. `h` and `rstd` are add_rms_norm's; dy, h and dh have one type.
     """
-    dtype, shape, dev = h.dtype, h.shape, h.device
-    code = DTYPE.get(dtype)
-    if code is None:
-        raise TypeError(f"h: expected fp16, bf16 or fp32, got {dtype}")
-    if not shape or shape[-1] < 1:
-        raise ValueError(f"h: expected shape [..., hidden] with hidden >= 1, got {tuple(shape)}")
-    hidden = shape[-1]
-    if dy.dtype != dtype or dy.shape != shape or dy.device != dev:
-        _like(dy, h, "dy")
-    if dh is not None and (dh.dtype != dtype or dh.shape != shape or dh.device != dev):
-        _like(dh, h, "dh")
-    wcode = _check_weight(weight, hidden, dtype, dev)
-    if rstd.dtype != torch.float32 or rstd.shape != shape[:-1] or not rstd.is_contiguous():
-        raise ValueError(f"rstd: expected {tuple(shape[:-1])} of torch.float32, contiguous")
-    if rstd.device != dev:
-        raise ValueError(f"rstd: on {rstd.device}, expected {dev}")
-    inner, outers, inners = _rows([dy, h] if dh is None else [dy, h, dh])
-    if dev.type != "cuda":
-        raise ValueError(f"the tensors must be on a CUDA device, got {dev}")
-    device, rows = dev.index, rstd.numel()
+    key = (_describe(dy), _describe(h), _describe(weight), _describe(rstd), None if dh is None else _describe(dh))
+    plan = _plans.get(key) or _keep(key, _plan_backward(dy, h, weight, rstd, dh))
     dx = torch.empty_like(h, memory_format=_CONTIGUOUS)
     dw = torch.empty_like(weight)
-    nbytes = _workspace_bytes(device, rows, hidden, code)
-    ws = _empty((nbytes // 4,), torch.float32, dev)
-    s = (dh.data_ptr(), outers[2], inners[2]) if dh is not None else (0, 0, 0)
-    err = C.create_string_buffer(_ERR)
+    ws = _empty((plan.nbytes // 4,), torch.float32, h.device)
+    err = emu.ERR.buf
+    (ydo, ydi), (ho, hi) = plan.strides
     rc = lib().nb_add_rms_norm_backward(
-        _BWD.pack(dy.data_ptr(), outers[0], inners[0], h.data_ptr(), outers[1], inners[1], *s, weight.data_ptr(),
-                  rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), nbytes, rows, inner, device, hidden,
-                  code, wcode),
-        emu.raw_stream(device), err, _ERR)
+        plan.pack(dy.data_ptr(), ydo, ydi, h.data_ptr(), ho, hi, 0 if dh is None else dh.data_ptr(), *plan.extra,
+                  weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), plan.nbytes,
+                  *plan.tail),
+        emu.raw_stream(plan.device), err, _ERR)
     if rc:
         _raise(err, rc)
     return dx, dw

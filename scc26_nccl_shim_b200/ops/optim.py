@@ -24,7 +24,7 @@ DTYPE = {torch.float16: 6, torch.float32: 7, torch.bfloat16: 9}
 E4M3 = torch.float8_e4m3fn
 NCCL_E4M3 = 10
 BLOCK = 256  # elements that share a scale in the 8-bit states
-_ERR = 256
+_ERR = emu.ERR.size
 
 
 class _Desc(C.Structure):  # nb_adamw_t
@@ -133,7 +133,7 @@ class GradNorm(_Bound):
         flat = [t for g in parts for t in g]
         super().__init__(first.device, flat)
         sizes = (C.c_uint64 * len(parts))(*[g[0].numel() for g in parts])
-        err = C.create_string_buffer(_ERR)
+        err = emu.ERR.buf
         self._handle = lib().nb_grad_norm_create(self._index, len(parts), len(parts[0]), DTYPE[first.dtype], sizes,
                                                  _addresses(flat), err, _ERR)
         if not self._handle:
@@ -150,7 +150,7 @@ class GradNorm(_Bound):
         self._check_storages()
         out = torch.empty_strided((2,), (1,), dtype=torch.float32, device=self.device)
         ws = torch.empty_strided((self._partials,), (1,), dtype=torch.float64, device=self.device)
-        err = C.create_string_buffer(_ERR)
+        err = emu.ERR.buf
         rc = lib().nb_grad_norm(self._handle, max_norm, scale, out.data_ptr(), ws.data_ptr(), emu.raw_stream(self._index),
                                 err, _ERR)
         if rc:
@@ -250,7 +250,7 @@ class AdamW(_Bound):
         desc = _Desc(self._index, len(params), len(parts[0]), DTYPE[first.dtype], DTYPE[gtype],
                      DTYPE[ctype] if ctype else 0, NCCL_E4M3 if self._eight else DTYPE[torch.float32],
                      seed & 0xFFFFFFFF, *[C.cast(t, C.c_void_p) if t is not None else None for t in tables], b1, b2, eps)
-        err = C.create_string_buffer(_ERR)
+        err = emu.ERR.buf
         self._handle = lib().nb_adamw_create(C.byref(desc), err, _ERR)
         if not self._handle:
             raise RuntimeError(err.value.decode())
@@ -280,7 +280,7 @@ class AdamW(_Bound):
         t, t_dev = self._scalar(t, "t", torch.int64)
         lr, lr_dev = self._scalar(lr, "lr", torch.float32)
         scale, scale_dev = self._scalar(scale, "scale", torch.float32)
-        err = C.create_string_buffer(_ERR)
+        err = emu.ERR.buf
         rc = lib().nb_adamw_step(self._handle, t, t_dev, lr, lr_dev, scale, scale_dev, emu.raw_stream(self._index), err, _ERR)
         if rc:
             raise (ValueError if rc == -1 else RuntimeError)(f"{err.value.decode()} ({rc})")

@@ -52,6 +52,27 @@ class OpDevice {
   bool switched_ = false;
 };
 
+// Lets `fn` have up to `bytes` of dynamic shared memory on `device` (the current
+// one): asked for once, since the call takes about a microsecond.
+inline cudaError_t op_allow_smem(const void* fn, int device, int bytes) {
+  constexpr int kSlots = 64;
+  static std::atomic<const void*> known[64][kSlots];
+  const bool keeps = device >= 0 && device < 64;
+  int slot = 0;
+  if (keeps)
+    for (; slot < kSlots; ++slot) {
+      const void* k = known[device][slot].load(std::memory_order_acquire);
+      if (k == fn) return cudaSuccess;
+      if (!k) break;
+    }
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && keeps && slot < kSlots) {
+    const void* none = nullptr;  // another thread may have taken the slot: then the next call asks again
+    known[device][slot].compare_exchange_strong(none, fn, std::memory_order_release);
+  }
+  return e;
+}
+
 // Launches a kernel that begins with op_wait_for_previous(): its blocks may be
 // set up while the stream's previous kernel ends.
 inline cudaError_t op_launch_after(const void* fn, dim3 grid, dim3 block, void** argv, cudaStream_t stream) {

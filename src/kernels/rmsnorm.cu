@@ -1045,11 +1045,11 @@ Shape shape_bwd(long long rows, int hidden, int es, bool vec, int sms) {
   }
   const int by_threads = (vec ? kRingThreads : kStagedThreads) / s.threads;
   const int by_smem = s.ring || s.staged ? int(size_t(kRingSmem) / s.smem) : by_threads;
-  // As many as are resident, but with four rows each before every SM has more
+  // As many as are resident, but with two rows each before every SM has more
   // than one; of a pair's blocks, half as many.
   const int places = s.pair ? sms / 2 > 0 ? sms / 2 : 1 : sms;
   const long long fit = (long long)places * (by_smem < by_threads ? by_smem : by_threads);
-  const long long most = ceil_div(rows, rows_per_block(s)), few = ceil_div(most, 4);
+  const long long most = ceil_div(rows, rows_per_block(s)), few = ceil_div(most, 2);
   s.blocks = most < places ? most : few < places ? places : few < fit ? few : fit;
   return s;
 }
@@ -1101,11 +1101,11 @@ const void* by_types(int dtype, bool wf32, F f) {
   }
 }
 
-cudaError_t launch(const void* fn, const Shape& s, unsigned blocks, void** argv, cudaStream_t stream) {
+cudaError_t launch(const void* fn, const Shape& s, int device, unsigned blocks, void** argv, cudaStream_t stream) {
   size_t smem = 0;
   if (s.ring || s.staged) {
     smem = s.smem;
-    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    const cudaError_t e = op_allow_smem(fn, device, kRingSmem);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg{};
@@ -1223,7 +1223,7 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   const void* fn = by_types(a->dtype, a->weight_dtype == NB_NORM_FLOAT32,
                             [&](auto kernels) { return kernels.fwd(f8, vec, a->parts > 1, s); });
   void* argv[] = {&k};
-  const cudaError_t e = launch(fn, s, unsigned(s.blocks), argv, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch(fn, s, a->device, unsigned(s.blocks), argv, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : op_refuse(err, errcap, "launch of the norm failed", int(e));
 }
 
@@ -1278,7 +1278,7 @@ extern "C" int nb_add_rms_norm_backward(const nb_norm_grad_t* a, void* stream, c
   if (a->rows) {
     const void* fn = by_types(a->dtype, a->weight_dtype == NB_NORM_FLOAT32,
                               [&](auto kernels) { return kernels.bwd(vec, s); });
-    e = launch(fn, s, unsigned(s.k ? parts : a->rows), argv, st);
+    e = launch(fn, s, a->device, unsigned(s.k ? parts : a->rows), argv, st);
     if (e == cudaSuccess && !s.k) {
       fn = a->dtype == NB_NORM_FLOAT32   ? pick_dw_long<float>(vec)
            : a->dtype == NB_NORM_FLOAT16 ? pick_dw_long<__half>(vec)
