@@ -27,8 +27,11 @@ namespace {
 using namespace octet;
 
 constexpr int kLongThreads = 1024;
-constexpr int kRingThreads = 512;    // a block of the gradient's kernels at most (128 registers each)
-constexpr int kStagedThreads = 640;  // of its staged form (102 registers): two blocks an SM for up to 5120 columns
+// A block of the gradient's kernels at most: 128 registers each (with 102 the
+// ring's spill, and took 148 us instead of 88); and of the staged ones, whose two
+// blocks an SM for up to 5120 columns have 51 or 102.
+constexpr int kRingThreads = 512;
+constexpr int kStagedThreads = 640;
 constexpr int kAll = 1 << 30;  // as what is left of a row: a store to shared memory that has room for everything
 // A block of the norm's at most: 64 registers do for one sum and its residual.
 __host__ __device__ constexpr int max_threads(bool many) { return many ? 512 : 1024; }
@@ -45,7 +48,7 @@ struct RowSplit {
 };
 
 struct FwdArgs {
-  Rows x[8];
+  Rows x[9];  // the partial sums, and the residual behind the last
   Rows residual;
   const void* weight;
   void* y;
@@ -243,19 +246,17 @@ struct Window {
   // `begin`: the tensor's first element. A piece that starts before it (the
   // first row's) is filled one element at a time.
   static __device__ __forceinline__ void fetch(T* to, const T* row, const T* begin, int hidden, int lane, int tpr) {
-    const int d = shift(row), pieces = (d + hidden + E - 1) / E;
-    for (int i = lane; i < pieces; i += tpr) {
-      const T* q = row - d + i * E;
-      if (q >= begin) {
-        const int rest = d + hidden - i * E, bytes = (rest < E ? rest : E) * int(sizeof(T));
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                         uint32_t(__cvta_generic_to_shared(to + i * E))),
-                     "l"(q), "r"(bytes)
-                     : "memory");
-      } else {
-        for (int e = d; e < E && e < d + hidden; ++e) to[i * E + e] = q[e];
-      }
-    }
+    const int d = shift(row), whole = (d + hidden) / E, tail = (d + hidden) % E;
+    const T* const from = row - d;
+    const bool inside = from >= begin;
+    const uint32_t at = uint32_t(__cvta_generic_to_shared(to));
+    for (int i = lane || inside ? lane : tpr; i < whole; i += tpr)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i * 16), "l"(from + i * E) : "memory");
+    if (tail && lane == whole % tpr && (whole || inside))
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + whole * 16), "l"(from + whole * E),
+                   "r"(tail * int(sizeof(T)))
+                   : "memory");
+    if (!inside && lane < E - d && lane < hidden) to[d + lane] = row[lane];
   }
 };
 
@@ -271,26 +272,24 @@ struct OutWindow {
 
   __device__ __forceinline__ int shift() const { return int(reinterpret_cast<uintptr_t>(to) & 15) / B; }
   __device__ __forceinline__ uint8_t* element(int i) const { return stage + (shift() + i) * B; }
+  __device__ __forceinline__ void put(int i) const {
+    if constexpr (B == 1) to[i] = *element(i);
+    else if constexpr (B == 2) reinterpret_cast<uint16_t*>(to)[i] = *reinterpret_cast<const uint16_t*>(element(i));
+    else reinterpret_cast<uint32_t*>(to)[i] = *reinterpret_cast<const uint32_t*>(element(i));
+  }
   __device__ __forceinline__ void flush(int hidden, int lane, int tpr) const {
-    const int d = shift(), pieces = (d + hidden + E - 1) / E;
-    for (int i = lane; i < pieces; i += tpr) {
-      const int first = i * E - d;  // the piece's first element
-      if (first >= 0 && first + E <= hidden) {
-        *reinterpret_cast<uint4*>(to + first * B) = *reinterpret_cast<const uint4*>(stage + i * 16);
-      } else {
-        for (int e = first < 0 ? 0 : first; e < first + E && e < hidden; ++e) {
-          if constexpr (B == 1) to[e] = *element(e);
-          else if constexpr (B == 2)
-            reinterpret_cast<uint16_t*>(to)[e] = *reinterpret_cast<const uint16_t*>(element(e));
-          else
-            reinterpret_cast<uint32_t*>(to)[e] = *reinterpret_cast<const uint32_t*>(element(e));
-        }
-      }
-    }
+    const int d = shift(), whole = (d + hidden) / E, tail = (d + hidden) % E;
+    uint8_t* const from = to - d * B;  // the first piece's place
+    for (int i = lane + (d ? 1 : 0); i < whole; i += tpr)
+      *reinterpret_cast<uint4*>(from + i * 16) = *reinterpret_cast<const uint4*>(stage + i * 16);
+    if (d && lane < E - d && lane < hidden) put(lane);
+    // The end, unless it is in the first piece.
+    if (lane < tail && (whole || !d)) put(hidden - tail + lane);
   }
 };
 
-// Elements of a row's window, which has room for all that its threads read.
+// Elements of a row's window, which has room for all that its threads read;
+// what lies behind the row is anything.
 template <typename T, int K>
 struct Staged {
   const T* base;  // the row's element 0
@@ -298,18 +297,21 @@ struct Staged {
 
   __device__ __forceinline__ void get(int k, Pair (&f)[4]) const {
     const T* p = base + part.at[k];
-    float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_float<T>(p[j * 32]);
-    if (part.left[k] <= 7 * 32) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j * 32 >= part.left[k]) v[j] = 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = pair(v[2 * j], v[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) f[j] = pair(to_float<T>(p[j * 64]), to_float<T>(p[j * 64 + 32]));
   }
 };
+
+// Zero where a thread's single elements lie behind the row.
+__device__ __forceinline__ void clear_behind(Pair (&f)[4], int left) {
+  if (left > 7 * 32) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float a, b;
+    split(f[j], a, b);
+    f[j] = pair(j * 64 < left ? a : 0.0f, j * 64 + 32 < left ? b : 0.0f);
+  }
+}
 
 // From the fp32 sum of a row to everything that is stored. part.left is 0 for
 // threads without a row. STAGED: the outputs go through `stage`, whose
@@ -397,6 +399,13 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool
 // first value is used, and a row's threads meet once (twice with one e4m3
 // scale per row). Octets on their boundary. W: the weight's type; MANY: more
 // than one partial sum.
+//
+// Two octets a thread share the cost of the row's sum: 8192 x 4096 bf16 with
+// residual takes 41.5 us (98 % of the copy bandwidth) against 46 with one octet.
+// Blocks that walk over rows with asynchronous copies ahead took 46.5 there, so a
+// row has a block. With e4m3 output the arithmetic behind the sum, a chain
+// of maximum, scale and conversion, shows: 16384 x 5120 in 105 us, 86 %.
+// One row of 8192 takes 2.8 us, most of it the launch.
 template <typename T, typename W, bool F8, bool MANY, int K>
 __global__ void __launch_bounds__(max_threads(MANY)) norm_kernel(const __grid_constant__ FwdArgs a) {
   __shared__ float red[32];
@@ -453,8 +462,11 @@ __global__ void __launch_bounds__(max_threads(MANY)) norm_kernel(const __grid_co
 // The same for rows off the vector boundary, which go through shared memory:
 // all sources of a row are on their way at once without a register held for
 // them, and single elements come out of shared memory. A row has a warp or a block.
+// Bound by the instructions that single elements take: 8192 x 4097 bf16 in 77 us
+// (single elements straight from memory: 106; octets cut out of the pieces
+// in registers: 142), four fp16 partials of 1013 x 5001 with e4m3 output in 22 us.
 template <typename T, typename W, bool F8, int K>
-__global__ void __launch_bounds__(512) norm_staged_kernel(const __grid_constant__ FwdArgs a) {
+__global__ void __launch_bounds__(kStagedThreads, 2) norm_staged_kernel(const __grid_constant__ FwdArgs a) {
   extern __shared__ uint4 smem[];
   __shared__ float red[32];
   __shared__ uint32_t top_red[32];
@@ -464,10 +476,8 @@ __global__ void __launch_bounds__(512) norm_staged_kernel(const __grid_constant_
   const Row from(row, a.split);
   const int sources = a.parts + (a.residual.p ? 1 : 0);
   T* const stage = reinterpret_cast<T*>(smem) + slot * a.windows * a.window;
-  for (int s = 0; s < sources; ++s) {
-    const Rows& t = s < a.parts ? a.x[s] : a.residual;
-    Window<T>::fetch(stage + s * a.window, from.of<T>(t), static_cast<const T*>(t.p), a.hidden, lane, tpr);
-  }
+  for (int s = 0; s < sources; ++s)
+    Window<T>::fetch(stage + s * a.window, from.of<T>(a.x[s]), static_cast<const T*>(a.x[s].p), a.hidden, lane, tpr);
   asm volatile("cp.async.commit_group;" ::: "memory");
   const Part<K, false> part(lane, tpr, a.hidden);
   Load<W, false, K> wv;
@@ -475,16 +485,23 @@ __global__ void __launch_bounds__(512) norm_staged_kernel(const __grid_constant_
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   row_sync(tpr);
   Pair h[K][4], f[4];
-  for (int s = 0; s < sources; ++s) {
-    const T* r = from.of<T>(s < a.parts ? a.x[s] : a.residual);
-    const Staged<T, K> v{stage + s * a.window + Window<T>::shift(r), part};
+  const auto source = [&](int i) {
+    return Staged<T, K>{stage + i * a.window + Window<T>::shift(from.of<T>(a.x[i])), part};
+  };
+  const Staged<T, K> first = source(0);
+#pragma unroll
+  for (int k = 0; k < K; ++k) first.get(k, h[k]);
+#pragma unroll 1
+  for (int i = 1; i < sources; ++i) {
+    const Staged<T, K> v = source(i);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       v.get(k, f);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) h[k][j] = s ? h[k][j] + f[j] : f[j];
+      add(h[k], f);
     }
   }
+#pragma unroll
+  for (int k = 0; k < K; ++k) clear_behind(h[k], part.left[k]);
   finish_row<T, F8, false, true, K>(a, row, true, part, h, wv, red, top_red, stage);
 }
 
@@ -497,7 +514,7 @@ __device__ __forceinline__ void sum8(const FwdArgs& a, const Row& from, const Pa
   v.get(0, h);
 #pragma unroll 1
   for (int s = 1; s < a.parts + (a.residual.p ? 1 : 0); ++s) {
-    v.load(from.of<T>(s < a.parts ? a.x[s] : a.residual), part);
+    v.load(from.of<T>(a.x[s]), part);
     v.get(0, f);
     add(h, f);
   }
@@ -596,6 +613,10 @@ __device__ __forceinline__ void finish_grad(const BwdArgs& a, bool live, const P
     dy.get(k, g[k]);
     h.get(k, n[k]);
     wv.get(k, w);
+    if constexpr (STAGED) {
+      clear_behind(g[k], part.left[k]);
+      clear_behind(n[k], part.left[k]);
+    }
     if (part.left[k] > 0 && live) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -660,7 +681,8 @@ __device__ __forceinline__ void clear(Pair (&acc)[K][4]) {
 }
 
 // Each block walks over rows and keeps its columns' part of dw in registers;
-// the parts go to `partial` and dw_kernel adds them in block order.
+// the parts go to `partial` and dw_kernel adds them in block order. fp32 rows
+// use this form: 8192 x 4096 in 88 us (93 % of the copy bandwidth).
 template <typename T, typename W, int K>
 __global__ void __launch_bounds__(kRingThreads) norm_backward_kernel(const __grid_constant__ BwdArgs a) {
   __shared__ float red[2][32];
@@ -738,6 +760,11 @@ __device__ __forceinline__ float pair_sum(float s, float* box, unsigned rank, in
 // thread without an octet or a row reads what the ring happens to hold and
 // drops it. PAIR: a row is shared by the two blocks of a cluster, half of the
 // octets each, because one block's registers do not hold it.
+//
+// A row's sum stands between its loads and its stores, so that without copies
+// ahead the memory idles while a block reduces: 16384 x 4096 bf16 in 88 us (92 %
+// of the copy bandwidth) against 113 without the ring. Rows of 16384 as pairs: 2048
+// of them in 81 us, 105 with two passes over the row.
 template <typename T, typename W, bool PAIR, int K, int STAGES>
 __global__ void __launch_bounds__(kRingThreads) norm_backward_ring_kernel(const __grid_constant__ BwdArgs a) {
   extern __shared__ uint4 smem[];
@@ -804,7 +831,8 @@ __global__ void __launch_bounds__(kRingThreads) norm_backward_ring_kernel(const 
 // The same for rows off the boundary, a warp or a block to each: the rows on
 // their way are windows that the row's threads share, so they meet between a
 // stage's copies and its use, and between its use and the next copies. dx has
-// a window of its own.
+// a window of its own. 8192 x 4097 bf16 in 104 us (169 with single elements
+// straight from and to memory).
 constexpr int kStagesOff = 3;
 
 template <typename T, typename W, int K>
@@ -983,7 +1011,6 @@ int pow2_at_least(int n) {
 }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-
 
 // `k` octets a thread; rows of up to 32 threads share a block: `warp` gives each a whole warp.
 void spread(Shape& s, int octets, int k, bool warp) {
@@ -1199,6 +1226,7 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   }
   if (a->r_outer < 0 || a->r_inner < 0) return op_refuse(err, errcap, kNegative);
   k.residual = {a->residual, a->r_outer, a->r_inner};
+  k.x[a->parts] = k.residual;
   if (a->residual) vec = vec && octets_fit(a->residual, a->r_outer, a->r_inner, es);
   vec = vec && octets_fit(a->y, 0, 0, f8 ? 1 : es) && (!a->h || octets_fit(a->h, 0, 0, es));
   const int sources = a->parts + (a->residual ? 1 : 0), outputs = a->h ? 2 : 1;
