@@ -7,7 +7,8 @@ provides the NCCL-ABI client, data generators, clock sampling and the
 formal-model checkers used by the tests and the benchmark.
 
 Subpackages:
-  ops/       ctypes bindings to the kernels (single-GPU virtual-rank runs)
+  ops/       ctypes bindings to the kernels: single-GPU virtual-rank runs (emu),
+             and the operators behind a reduction (norm, optim)
   parallel/  the NCCL C ABI client (comm init, grouped collectives)
   utils/     seeded data, clock sampling, timing helpers
   models/    explicit-state checkers of the GroupFallback / HostLaneReuse models

@@ -462,9 +462,9 @@ __global__ void __launch_bounds__(max_threads(MANY)) norm_kernel(const __grid_co
 // The same for rows off the vector boundary, which go through shared memory:
 // all sources of a row are on their way at once without a register held for
 // them, and single elements come out of shared memory. A row has a warp or a block.
-// Bound by the instructions that single elements take: 8192 x 4097 bf16 in 77 us
+// Bound by the instructions that single elements take: 8192 x 4097 bf16 in 76 us
 // (single elements straight from memory: 106; octets cut out of the pieces
-// in registers: 142), four fp16 partials of 1013 x 5001 with e4m3 output in 22 us.
+// in registers: 142), four fp16 partials of 1013 x 5001 with e4m3 output in 21 us.
 template <typename T, typename W, bool F8, int K>
 __global__ void __launch_bounds__(kStagedThreads, 2) norm_staged_kernel(const __grid_constant__ FwdArgs a) {
   extern __shared__ uint4 smem[];
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(kRingThreads) norm_backward_ring_kernel(const 
 // The same for rows off the boundary, a warp or a block to each: the rows on
 // their way are windows that the row's threads share, so they meet between a
 // stage's copies and its use, and between its use and the next copies. dx has
-// a window of its own. 8192 x 4097 bf16 in 104 us (169 with single elements
+// a window of its own. 8192 x 4097 bf16 in 102 us (169 with single elements
 // straight from and to memory).
 constexpr int kStagesOff = 3;
 
