@@ -696,10 +696,6 @@ extern "C" int nb_adamw_step(const void* handle, int64_t t, const int64_t* t_dev
   const AdamHandle* h = static_cast<const AdamHandle*>(handle);
   if (!h || h->magic != kAdamMagic) return op_refuse(err, errcap, "bad arguments: not an AdamW handle");
   if (!t_dev && t < 1) return op_refuse(err, errcap, "bad arguments: steps count from 1");
-  if (!lr_dev && !std::isfinite(lr)) return op_refuse(err, errcap, "bad arguments: lr must be finite");
-  if (!std::isfinite(scale)) return op_refuse(err, errcap, "bad arguments: scale must be finite");
-  OpDevice dev(h->device);
-  if (dev.error()) return op_refuse(err, errcap, "cannot use the device", int(dev.error()));
   StepScalars s{};
   s.t = reinterpret_cast<const long long*>(t_dev);
   s.lr = lr_dev;
@@ -713,6 +709,12 @@ extern "C" int nb_adamw_step(const void* handle, int64_t t, const int64_t* t_dev
     s.t_lr_m = float(lr * inv1);
     s.t_root = float(1.0 / std::sqrt(-std::expm1(double(t) * std::log(h->beta2))));
   }
+  // Checked as the kernel gets them: past fp32's range they would be infinite there.
+  if (!lr_dev && (!std::isfinite(s.lr_host) || !std::isfinite(s.t_lr_m)))
+    return op_refuse(err, errcap, "bad arguments: lr, and lr / (1 - beta1^t), must be finite in fp32");
+  if (!std::isfinite(s.scale_host)) return op_refuse(err, errcap, "bad arguments: scale must be finite in fp32");
+  OpDevice dev(h->device);
+  if (dev.error()) return op_refuse(err, errcap, "cannot use the device", int(dev.error()));
   const auto fill = [&](auto& k) {
     k.s = s;
     k.b1 = float(h->beta1);
@@ -794,7 +796,8 @@ extern "C" int nb_grad_norm(const void* handle, double max_norm, double scale, f
   const NormHandle* h = static_cast<const NormHandle*>(handle);
   if (!h || h->magic != kNormMagic) return op_refuse(err, errcap, "bad arguments: not a gradient norm's handle");
   if (!(max_norm > 0)) return op_refuse(err, errcap, "bad arguments: max_norm must be positive");
-  if (!(scale > 0) || !std::isfinite(scale)) return op_refuse(err, errcap, "bad arguments: scale must be positive");
+  if (!(scale > 0) || !std::isfinite(float(scale)))
+    return op_refuse(err, errcap, "bad arguments: scale must be positive, and finite in fp32");
   if (!out || !on_boundary(out, 4) || (h->partials && (!workspace || !on_boundary(workspace, 8))))
     return op_refuse(err, errcap, "bad arguments: null or misaligned output or workspace");
   OpDevice dev(h->device);

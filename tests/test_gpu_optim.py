@@ -440,6 +440,22 @@ def test_refused_steps_change_nothing():
     assert torch.equal(p, held)
 
 
+def test_numbers_beyond_fp32_are_refused():
+    m = optim()
+    p, g = data(100, torch.float32, 1), data(100, torch.float32, 2)
+    opt = m.AdamW([p], [g], betas=(0.999, 0.999))
+    held = p.clone()
+    # 1e37 is one, 1e37 / (1 - 0.999) is not.
+    for kw in (dict(t=1, lr=1e39), dict(t=1, lr=1e37), dict(t=1, lr=LR, scale=1e39),
+               dict(t=torch.ones(1, dtype=torch.int64, device=DEV), lr=1e39)):
+        with pytest.raises(ValueError, match="fp32"):
+            opt.step(**kw)
+    assert torch.equal(p, held)
+    for norm_of in (dict(scale=math.inf), dict(scale=1e39), dict(max_norm=0.0), dict(max_norm=math.nan)):
+        with pytest.raises(ValueError):
+            m.GradNorm([g])(**norm_of)
+
+
 def test_guards_around_every_tensor():
     m = optim()
     sizes = [5, 300, 2049]
