@@ -133,7 +133,7 @@ def _like(t: torch.Tensor, ref: torch.Tensor, name: str) -> None:
 
 
 def _raise(err, rc: int) -> None:
-    raise RuntimeError(f"{err.value.decode()} ({rc})")
+    raise (ValueError if rc == -1 else RuntimeError)(f"{err.value.decode()} ({rc})")
 
 
 def _empty(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
@@ -195,8 +195,8 @@ def _plan_forward(xs: list, weight: torch.Tensor, residual: torch.Tensor | None,
         raise TypeError(f"out_dtype: expected {dtype} or {E4M3}, got {out_dtype}")
     if group not in GROUPS or (group and not f8):
         raise ValueError(f"group: one of {GROUPS} with e4m3 output, else 0, got {group}")
-    if not 0 < eps < math.inf:
-        raise ValueError(f"eps: must be positive, got {eps}")
+    if not 1.2e-38 <= eps <= 3.4e38:
+        raise ValueError(f"eps: must be a positive normal fp32 number, got {eps}")
     inner, outers, inners = _rows(xs if residual is None else xs + [residual])
     device = dev.index if dev.type == "cuda" else -1
     return _Plan(_FWD[n].pack, (*outers[:n], *inners[:n]), (outers[n], inners[n]) if residual is not None else (0, 0),

@@ -134,6 +134,12 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+@pytest.mark.parametrize("eps", [1e-50, 1e-42, 1e39, -1e-6, float("inf")])
+def test_norm_refuses_an_eps_beyond_fp32(eps):
+    with pytest.raises(ValueError, match="eps"):
+        norm.add_rms_norm(x(4, 64), W, eps=eps)
+
+
 def test_c_entry_points_refuse_with_a_message():
     """The C ABI's own checks, without a device."""
     L, err = norm.lib(), C.create_string_buffer(256)
