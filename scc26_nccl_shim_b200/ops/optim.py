@@ -110,6 +110,9 @@ class _Bound:
         self._storages = list(storages.values())
         self._where = list(storages)
 
+    def __reduce_ex__(self, protocol):  # a copy would share the handle, and its tensors would not be the handle's
+        raise TypeError(f"{type(self).__name__} is bound to its tensors: make a new one instead of copying it")
+
     def _check_storages(self) -> None:
         if [s.data_ptr() for s in self._storages] != self._where:
             raise RuntimeError("a tensor's storage was resized or moved since this was made")
@@ -172,8 +175,10 @@ class AdamW(_Bound):
     `state="float32"`: `exp_avg`, `exp_avg_sq` are fp32 tensors. `state="8bit"`:
     they are pairs (e4m3 codes, fp32 scale per block of 256 elements), of m and
     of sqrt(v), rounded at random with bits that are a hash of (`seed`, t, tensor,
-    element); `moments(i)` gives their values. `states=(exp_avg, exp_avg_sq)`
-    takes given ones instead of zeros (to resume).
+    element); `moments(i)` gives their values. A gradient that is not finite
+    spoils the states of its block, as one of its element in fp32: clip with
+    GradNorm's coefficient, which skips such a step. `states=(exp_avg,
+    exp_avg_sq)` takes given ones instead of zeros (to resume).
 
     The tensors are bound by their memory: give new ones (after `.data =` or a
     resize) to a new AdamW. No two of them may overlap where one is written.

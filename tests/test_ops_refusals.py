@@ -1,6 +1,8 @@
 """What the norm and optimizer operators refuse (CPU): every check of types,
 shapes, strides and overlaps is made before the device is looked at."""
+import copy
 import ctypes as C
+import pickle
 
 import pytest
 import torch
@@ -138,6 +140,15 @@ def test_cpu_tensors_are_refused():
 def test_norm_refuses_an_eps_beyond_fp32(eps):
     with pytest.raises(ValueError, match="eps"):
         norm.add_rms_norm(x(4, 64), W, eps=eps)
+
+
+@pytest.mark.parametrize("cls", [optim.AdamW, optim.GradNorm])
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, pickle.dumps])
+def test_bound_tensors_are_not_copied(cls, how):
+    bound = cls.__new__(cls)  # what is refused does not depend on the tensors
+    bound._handle = 1
+    with pytest.raises(TypeError, match="make a new one"):
+        how(bound)
 
 
 def test_c_entry_points_refuse_with_a_message():
