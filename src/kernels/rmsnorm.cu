@@ -33,8 +33,16 @@ constexpr int kLongThreads = 1024;
 constexpr int kRingThreads = 512;
 constexpr int kStagedThreads = 640;
 constexpr int kAll = 1 << 30;  // as what is left of a row: a store to shared memory that has room for everything
-// A block of the norm's at most: 64 registers do for one sum and its residual.
-__host__ __device__ constexpr int max_threads(bool many) { return many ? 512 : 1024; }
+
+// Registers of a thread of the norm's kernel. A row's loads, its sum and its
+// stores follow one another, so what keeps HBM busy is how many rows an SM holds,
+// and these decide that (see shape_fwd, which picks a variant; times there). es,
+// ws: bytes of the input's and the weight's elements.
+__host__ __device__ constexpr int norm_registers(int es, int ws, int at_once, int k, bool pair, bool lean) {
+  if (es == 4 || k == 1) return at_once == 1 ? 64 : 128;
+  if (ws == 4) return at_once == 4 ? 96 : at_once == 2 && pair ? 72 : 64;
+  return at_once == 4 ? (lean ? 72 : 80) : at_once == 2 ? (pair ? 64 : 56) : lean ? 40 : 48;
+}
 
 struct Rows {
   const void* p;
@@ -59,6 +67,7 @@ struct FwdArgs {
   RowSplit split;
   int hidden, parts, group, group_log, tpr, groups;
   int window, windows;  // elements between staged rows, and a row's number of them
+  int half;             // columns of a pair's first block
   float eps, inv_hidden;
 };
 
@@ -313,14 +322,42 @@ __device__ __forceinline__ void clear_behind(Pair (&f)[4], int left) {
   }
 }
 
+// What the other block of a cluster of two gives: each stores its own where
+// the other reads it. `box`: a word of shared memory that is not written again before
+// both have read it (the next exchange's is another one).
+__device__ __forceinline__ uint32_t pair_other(uint32_t mine, float* box, unsigned rank) {
+  const uint32_t at = uint32_t(__cvta_generic_to_shared(box));
+  if (threadIdx.x == 0) {
+    uint32_t far;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(at), "r"(rank ^ 1u));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(far), "r"(mine) : "memory");
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  return *reinterpret_cast<volatile uint32_t*>(box);
+}
+
+// The sum of a value of each of the two blocks of a cluster, the same in both.
+__device__ __forceinline__ float pair_sum(float s, float* box, unsigned rank, int turn) {
+  const float other = __uint_as_float(pair_other(__float_as_uint(s), box + (turn & 1), rank));
+  return rank ? other + s : s + other;
+}
+
+// A block's half of a row that two share: from which column on, and which of
+// the two. Elsewhere all of it.
+struct Half {
+  int from = 0;
+  unsigned rank = 0;
+  float* box = nullptr;  // two words, for the sum and the maximum
+};
+
 // From the fp32 sum of a row to everything that is stored. part.left is 0 for
 // threads without a row. STAGED: the outputs go through `stage`, whose
 // contents (the sources) every thread has read.
-template <typename T, bool F8, bool VEC, bool STAGED, int K, typename Weight>
+template <typename T, bool F8, bool VEC, bool STAGED, bool PAIR, int K, typename Weight>
 __device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool live,
                                            const Part<K, VEC>& part,
                                            const Pair (&h)[K][4], const Weight& wv, float* red, uint32_t* top_red,
-                                           T* stage = nullptr) {
+                                           const Half& half, T* stage = nullptr) {
   const int tpr = a.tpr;
   Pair sum = pair(0.0f, 0.0f), f[4];
 #pragma unroll
@@ -329,7 +366,7 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum = fma(h[k][j], h[k][j], sum);
     }
-  const long long out = row * a.hidden;
+  const long long out = row * a.hidden + (PAIR ? half.from : 0);
   const OutWindow<int(sizeof(T))> hw{reinterpret_cast<uint8_t*>(static_cast<T*>(a.h) + out),
                                      reinterpret_cast<uint8_t*>(stage)};
   const OutWindow<F8 ? 1 : int(sizeof(T))> yw{static_cast<uint8_t*>(a.y) + out * (F8 ? 1 : int(sizeof(T))),
@@ -347,9 +384,14 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool
     }
   };
   if constexpr (!STAGED) put_h();
-  const float s = row_sum(sum_of(sum), tpr, red);
+  float s = row_sum(sum_of(sum), tpr, red);
+  if constexpr (PAIR) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the other block has started
+    s = pair_sum(s, half.box, half.rank, 0);
+  }
   const float rstd = rsqrtf(fmaf(s, a.inv_hidden, a.eps));
-  if (live && part.lane == 0) a.rstd[row] = rstd;
+  const bool first = live && part.lane == 0 && (!PAIR || half.rank == 0);
+  if (first) a.rstd[row] = rstd;
   if constexpr (STAGED) {  // behind every thread's last read of a source
     if (tpr <= 32) __syncwarp();  // else row_sum has a barrier
     put_h();
@@ -377,14 +419,17 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool
     }
     float inv[8];
     if (a.group == 0) {
-      const float scale = scale_of(row_max(most, tpr, top_red));
-      if (live && part.lane == 0) a.scale[row] = scale;
+      most = row_max(most, tpr, top_red);
+      if constexpr (PAIR) most = max(most, pair_other(most, half.box + 1, half.rank));
+      const float scale = scale_of(most);
+      if (first) a.scale[row] = scale;
 #pragma unroll
       for (int j = 0; j < 8; ++j) inv[j] = reciprocal(scale);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (a.group) group_scales<VEC>(a, y[k], most, tpr, row, part.at[k], part.left[k], inv);
+      if (a.group)
+        group_scales<VEC>(a, y[k], most, tpr, row, (PAIR ? half.from : 0) + part.at[k], part.left[k], inv);
       store_e4m3<VEC>(y0 + part.at[k], y[k], inv, part.kStep, STAGED ? kAll : part.left[k]);
     }
   }
@@ -406,29 +451,44 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool
 // row has a block. With e4m3 output the arithmetic behind the sum, a chain
 // of maximum, scale and conversion, shows: 16384 x 5120 in 105 us, 86 %.
 // One row of 8192 takes 2.8 us, most of it the launch.
-template <typename T, typename W, bool F8, bool MANY, int K>
-__global__ void __launch_bounds__(max_threads(MANY)) norm_kernel(const __grid_constant__ FwdArgs a) {
+// PAIR: a row is shared by the two blocks of a cluster. Their part of it is a
+// multiple of 128 columns, so that no group of columns is in both.
+template <typename T, typename W, bool F8, int AT_ONCE, int K, bool PAIR = false, bool LEAN = false>
+__global__ void __maxnreg__(norm_registers(sizeof(T), sizeof(W), AT_ONCE, K, PAIR, LEAN))
+    norm_kernel(const __grid_constant__ FwdArgs a) {
   __shared__ float red[32];
   __shared__ uint32_t top_red[32];
+  __shared__ float box[2];
+  Half half;
+  int columns = a.hidden;
+  if constexpr (PAIR) {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    half.rank = blockIdx.x & 1;
+    half.box = box;
+    half.from = half.rank ? a.half : 0;
+    columns = half.rank ? a.hidden - a.half : a.half;
+  }
   const int tpr = a.tpr;
   const int lane = tpr > 32 ? threadIdx.x : threadIdx.x & (tpr - 1);
-  const long long row = tpr > 32 ? (long long)blockIdx.x
-                                 : (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+  const long long row = PAIR       ? (long long)(blockIdx.x >> 1)
+                        : tpr > 32 ? (long long)blockIdx.x
+                                   : (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
   const bool live = row < a.rows;  // every thread stays for the shuffles
   const Row from(live ? row : 0, a.split);
-  Part<K, true> part(lane, tpr, a.hidden);
-  // Four partial sums at a time, with the first of them the residual too.
-  constexpr int N = MANY ? 4 : 1;
+  Part<K, true> part(lane, tpr, columns);
+  const int at = PAIR ? half.from : 0;
+  // AT_ONCE partial sums at a time, with the first of them the residual too.
+  constexpr int N = AT_ONCE;
   Load<T, true, K> xv[N], rv;
   Load<W, true, K> wv;
   Pair h[K][4], f[4];
 #pragma unroll 1
-  for (int s0 = 0; s0 < (MANY ? a.parts : 1); s0 += N) {
+  for (int s0 = 0; s0 < (N > 1 ? a.parts : 1); s0 += N) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (s0 + i < a.parts) xv[i].load(from.of<T>(a.x[s0 + i]), part);
-    if (s0 == 0 && a.residual.p) rv.load(from.of<T>(a.residual), part);
-    if (s0 == 0) wv.load(static_cast<const W*>(a.weight), part);
+      if (s0 + i < a.parts) xv[i].load(from.of<T>(a.x[s0 + i]) + at, part);
+    if (s0 == 0 && a.residual.p) rv.load(from.of<T>(a.residual) + at, part);
+    if (s0 == 0) wv.load(static_cast<const W*>(a.weight) + at, part);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (s0 == 0) {
@@ -456,7 +516,7 @@ __global__ void __launch_bounds__(max_threads(MANY)) norm_kernel(const __grid_co
 #pragma unroll
     for (int k = 0; k < K; ++k) part.left[k] = 0;
   }
-  finish_row<T, F8, true, false, K>(a, row, live, part, h, wv, red, top_red);
+  finish_row<T, F8, true, false, PAIR, K>(a, row, live, part, h, wv, red, top_red, half);
 }
 
 // The same for rows off the vector boundary, which go through shared memory:
@@ -502,7 +562,7 @@ __global__ void __launch_bounds__(kStagedThreads, 2) norm_staged_kernel(const __
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) clear_behind(h[k], part.left[k]);
-  finish_row<T, F8, false, true, K>(a, row, true, part, h, wv, red, top_red, stage);
+  finish_row<T, F8, false, true, false, K>(a, row, true, part, h, wv, red, top_red, Half(), stage);
 }
 
 // The sum of every partial and the residual at eight elements.
@@ -739,22 +799,6 @@ struct Ring {
     for (int k = 0; k < K; ++k) o.raw[k].o.v[0] = *slot(stage, source, k);
   }
 };
-
-// The sum of a value of each of the two blocks of a cluster, the same in
-// both: each stores its own where the other reads it. `box`: two floats of
-// shared memory, used in turn, so that one is read while the other is written.
-__device__ __forceinline__ float pair_sum(float s, float* box, unsigned rank, int turn) {
-  if (threadIdx.x == 0) {
-    uint32_t far;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;"
-        : "=r"(far)
-        : "r"(uint32_t(__cvta_generic_to_shared(box + (turn & 1)))), "r"(rank ^ 1u));
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(far), "f"(s) : "memory");
-  }
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  const float other = *reinterpret_cast<volatile float*>(box + (turn & 1));
-  return rank ? other + s : s + other;
-}
 
 // The same with the next rows on their way (octets on their boundary). A
 // thread without an octet or a row reads what the ring happens to hold and
@@ -999,7 +1043,8 @@ constexpr int kRingSmem = 220 * 1024;  // of an SM's shared memory, for the ring
 // How rows are spread over threads and blocks.
 struct Shape {
   int tpr = 0, threads = 0, k = 0;  // k 0: the long variant
-  bool ring = false, staged = false, pair = false;
+  int at_once = 1, half = 0;  // partial sums at a time; columns of a pair's first block
+  bool ring = false, staged = false, pair = false, lean = false;
   size_t smem = 0;
   long long blocks = 0;
 };
@@ -1028,24 +1073,74 @@ int rows_per_block(const Shape& s) { return s.tpr > 32 ? 1 : s.threads / s.tpr; 
 // Elements from one staged row to the next: room for every thread's elements, and a piece more for its shift.
 int window_of(const Shape& s, int es) { return s.tpr * 8 * s.k + 16 / es; }
 
+// Blocks that an SM's registers hold: each of its four parts has 16384, and
+// takes a quarter of a block's warps or one more.
+int blocks_by_registers(int threads, int registers) { return 4 * (16384 / (32 * registers)) / (threads / 32); }
+
 // Aligned rows stay in registers; others go through shared memory, `windows`
 // (sources or outputs) of them for each row, where two blocks fit an SM. What
 // is too long for either is read again in each pass.
-Shape shape_fwd(long long rows, int hidden, int es, int windows, bool vec, bool many, int sms) {
+//
+// Of a row in registers, the variant that lets an SM hold two blocks at least
+// (norm_registers; bf16 with residual; "48 -> 40" are registers a thread):
+//  - one sum: 40 registers, which spill a few addresses, only where they hold more
+//    blocks: 4096 x 12288 with e4m3 output 84 -> 63 us, 8192 x 8192 88 -> 79; but
+//    16384 x 5120, where they do not, takes 100 instead of 94.
+//  - several: four at a time, or two where four leave one block (8192 x 8192, 8 sums:
+//    256 -> 226 us) or where there are two (8192 x 7168: 142 -> 92); four in 72
+//    registers for 80 where that holds more (8192 x 7168, 4 sums: 163 -> 117).
+//  - a pair of blocks for each row where one leaves no room for a second: 4096 x 16384
+//    96 -> 91 us, 4096 x 12288 with 8 sums 201 -> 172, and what one block does not hold:
+//    2048 x 20480 74 -> 63 (reading it again), 2048 x 16384 fp32 with 4 sums 211 -> 142.
+//    Not two sums at a time where a pair holds no more threads (4096 x 12288: 94 us, pairs
+//    104), nor one scale a row, whose maximum is a second meeting of the two (4096 x
+//    16384: 99 us, pairs 104); nor fp32 with fewer than three sums (2048 x 12288: 96
+//    us by reading again, pairs 102).
+// Up to a row an SM, one octet a thread is the shortest way.
+Shape shape_fwd(long long rows, int hidden, int es, int ws, int windows, bool vec, int parts, bool by_row, int sms) {
   Shape s;
-  const int octets = int(ceil_div(hidden, 8)), most = vec ? max_threads(many) : 512;
-  s.blocks = rows;
-  if (octets > 2 * most) return s;
-  spread(s, octets, octets > most || (vec ? rows > sms : octets > 32) ? 2 : 1, !vec);
-  s.blocks = ceil_div(rows, rows_per_block(s));
+  const int octets = int(ceil_div(hidden, 8));
+  s.at_once = parts == 1 ? 1 : 4;
   if (!vec) {
+    s.blocks = rows;
+    if (octets > 2 * 512) return s;
+    spread(s, octets, octets > 32 ? 2 : 1, true);
     s.staged = true;
     s.smem = size_t(rows_per_block(s)) * size_t(windows) * size_t(window_of(s, es)) * size_t(es);
-    if (s.smem > size_t(kRingSmem) / 2) {
-      s = Shape{};
-      s.blocks = rows;
+    if (s.smem > size_t(kRingSmem) / 2) s = Shape{};
+    s.blocks = s.k ? ceil_div(rows, rows_per_block(s)) : rows;
+    return s;
+  }
+  if (rows <= sms && octets <= (parts == 1 ? 1024 : 512)) {
+    spread(s, octets, 1, false);
+    s.blocks = ceil_div(rows, rows_per_block(s));
+    return s;
+  }
+  // One block a row, if two fit an SM; else a pair's two, where that pays; else one.
+  int alone = 0;
+  for (const int turn : {0, 1, 2}) {
+    s.pair = turn == 1;
+    s.half = s.pair ? int(ceil_div(octets, 32)) * 16 * 8 : hidden;
+    spread(s, s.half / 8, 2, false);
+    const auto fit = [&](int at_once, bool lean) {
+      return blocks_by_registers(s.threads, norm_registers(es, ws, at_once, 2, s.pair, lean));
+    };
+    const bool narrow = es == 2 && ws == 2;
+    if (parts > 1 && es == 2)
+      s.at_once = parts == 2 || s.threads > 512 || (rows > sms && fit(4, narrow) < 2) ? 2 : 4;
+    s.lean = narrow && s.at_once != 2 && fit(s.at_once, true) > fit(s.at_once, false);
+    const int blocks = fit(s.at_once, s.lean);
+    if (turn == 0 && s.threads <= 1024) alone = blocks * s.threads;
+    bool take = s.threads <= 1024 && blocks > (turn == 2 || es == 4 || rows <= sms ? 0 : 1);
+    if (s.pair && es == 4) take = take && parts > 2;
+    else if (s.pair) take = take && !(by_row && alone) && (s.at_once != 2 || blocks * s.threads > alone);
+    if (take) {
+      s.blocks = ceil_div(rows, rows_per_block(s));
+      return s;
     }
   }
+  s = Shape{};
+  s.blocks = rows;
   return s;
 }
 
@@ -1090,14 +1185,24 @@ RowSplit split_by(long long inner) {
   return s;
 }
 
+template <typename T, typename W, bool F8, bool PAIR>
+const void* fwd_kernel2(const Shape& s) {
+  if constexpr (sizeof(T) == 2)
+    if (s.at_once == 2) return reinterpret_cast<const void*>(norm_kernel<T, W, F8, 2, 2, PAIR>);
+  if constexpr (sizeof(T) == 2 && sizeof(W) == 2)
+    if (s.lean) return s.at_once == 4 ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, 4, 2, PAIR, true>)
+                                      : reinterpret_cast<const void*>(norm_kernel<T, W, F8, 1, 2, PAIR, true>);
+  return s.at_once == 4 ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, 4, 2, PAIR>)
+                        : reinterpret_cast<const void*>(norm_kernel<T, W, F8, 1, 2, PAIR>);
+}
+
 template <typename T, typename W, bool F8>
-const void* fwd_kernel(bool vec, bool many, const Shape& s) {
+const void* fwd_kernel(bool vec, const Shape& s) {
   if (s.staged) return s.k == 1 ? reinterpret_cast<const void*>(norm_staged_kernel<T, W, F8, 1>)
                                 : reinterpret_cast<const void*>(norm_staged_kernel<T, W, F8, 2>);
-  if (s.k == 1) return many ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, true, 1>)
-                            : reinterpret_cast<const void*>(norm_kernel<T, W, F8, false, 1>);
-  if (s.k == 2) return many ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, true, 2>)
-                            : reinterpret_cast<const void*>(norm_kernel<T, W, F8, false, 2>);
+  if (s.k == 1) return s.at_once == 4 ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, 4, 1>)
+                                      : reinterpret_cast<const void*>(norm_kernel<T, W, F8, 1, 1>);
+  if (s.k == 2) return s.pair ? fwd_kernel2<T, W, F8, true>(s) : fwd_kernel2<T, W, F8, false>(s);
   return vec ? reinterpret_cast<const void*>(norm_long_kernel<T, W, F8, true>)
              : reinterpret_cast<const void*>(norm_long_kernel<T, W, F8, false>);
 }
@@ -1105,8 +1210,8 @@ const void* fwd_kernel(bool vec, bool many, const Shape& s) {
 // The kernels of an input and a weight type.
 template <typename T, typename W>
 struct Kernels {
-  static const void* fwd(bool f8, bool vec, bool many, const Shape& s) {
-    return f8 ? fwd_kernel<T, W, true>(vec, many, s) : fwd_kernel<T, W, false>(vec, many, s);
+  static const void* fwd(bool f8, bool vec, const Shape& s) {
+    return f8 ? fwd_kernel<T, W, true>(vec, s) : fwd_kernel<T, W, false>(vec, s);
   }
   static const void* bwd(bool vec, const Shape& s) {
     if constexpr (sizeof(T) == 2)
@@ -1231,7 +1336,9 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   vec = vec && octets_fit(a->y, 0, 0, f8 ? 1 : es) && (!a->h || octets_fit(a->h, 0, 0, es));
   const int sources = a->parts + (a->residual ? 1 : 0), outputs = a->h ? 2 : 1;
   k.windows = sources > outputs ? sources : outputs;
-  const Shape s = shape_fwd(a->rows, a->hidden, es, k.windows, vec, a->parts > 1, dev.sms());
+  const Shape s =
+      shape_fwd(a->rows, a->hidden, es, size_of(a->weight_dtype), k.windows, vec, a->parts, f8 && !a->group, dev.sms());
+  k.half = s.half;
   k.weight = a->weight;
   k.y = a->y;
   k.scale = a->scale;
@@ -1249,7 +1356,7 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   k.eps = a->eps;
   k.inv_hidden = 1.0f / float(a->hidden);
   const void* fn = by_types(a->dtype, a->weight_dtype == NB_NORM_FLOAT32,
-                            [&](auto kernels) { return kernels.fwd(f8, vec, a->parts > 1, s); });
+                            [&](auto kernels) { return kernels.fwd(f8, vec, s); });
   void* argv[] = {&k};
   const cudaError_t e = launch(fn, s, a->device, unsigned(s.blocks), argv, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? 0 : op_refuse(err, errcap, "launch of the norm failed", int(e));

@@ -126,6 +126,27 @@ def test_many_rows(rows, hidden, dtype):
     assert torch.equal(got.y, want.y) and torch.equal(res, want.h)
 
 
+# Rows of one block, of two that share a row, and of 1, 2 and 4 sums at a time: on
+# both sides of the widths where that changes.
+WIDE = [(5, 8200), (300, 4608), (300, 7168), (200, 8960), (180, 9216), (200, 9224), (160, 10240), (170, 12296),
+        (150, 14336), (149, 16392), (150, 20480), (3, 24584), (149, 28672), (2, 32768), (149, 32776)]
+
+
+@pytest.mark.parametrize("parts", [1, 2, 3, 5])
+@pytest.mark.parametrize("rows, hidden", WIDE)
+def test_wide_rows(rows, hidden, parts):
+    m = norm()
+    for dtype, wtype in ((torch.bfloat16,) * 2, (torch.float16, torch.float32), (torch.float32,) * 2):
+        xs = [data((rows, hidden), dtype, k) for k in range(parts)]
+        res, w = data((rows, hidden), dtype, 9, 2.0), data((hidden,), wtype, 3)
+        want = m.add_rms_norm(xs, w, res)
+        check(want, xs, w, res, 1e-6)
+        for group in (0, 32, 128):
+            check(m.add_rms_norm(xs, w, out_dtype=E4M3, group=group), xs, w, None, 1e-6, group)
+        got = m.add_rms_norm(xs, w, res, out=m.NormOut(torch.empty_like(res), None, res, torch.empty_like(want.rstd)))
+        assert torch.equal(got.y, want.y) and torch.equal(res, want.h) and torch.equal(got.rstd, want.rstd)
+
+
 def test_sum_has_the_bits_of_the_collectives_fold():
     m = norm()
     from scc26_nccl_shim_b200.ops import emu
