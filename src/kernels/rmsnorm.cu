@@ -15,6 +15,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 #include <cstdio>
 
 #include "kernels/octet.cuh"
@@ -36,13 +37,20 @@ constexpr int kAll = 1 << 30;  // as what is left of a row: a store to shared me
 
 // Registers of a thread of the norm's kernel. A row's loads, its sum and its
 // stores follow one another, so what keeps HBM busy is how many rows an SM holds,
-// and these decide that (see shape_fwd, which picks a variant; times there). es,
-// ws: bytes of the input's and the weight's elements.
-__host__ __device__ constexpr int norm_registers(int es, int ws, int at_once, int k, bool pair, bool lean) {
+// and these decide that (see shape_fwd, which picks a variant; times there). es:
+// bytes of an input's element.
+__host__ __device__ constexpr int norm_registers(int es, int at_once, int k, bool pair, bool lean) {
   if (es == 4 || k == 1) return at_once == 1 ? 64 : 128;
-  if (ws == 4) return at_once == 4 ? 96 : at_once == 2 && pair ? 72 : 64;
   return at_once == 4 ? (lean ? 72 : 80) : at_once == 2 ? (pair ? 64 : 56) : lean ? 40 : 48;
 }
+
+// Where the weight is loaded behind the row's sum. Of 16-bit rows an fp32 one
+// takes a third of the registers: 16384 x 5120 bf16 to e4m3 in 93 us, 105 with the
+// weight loaded first. A 16-bit one beside a single sum makes 40 registers spill:
+// 8192 x 8192 to e4m3 80 against 85 us, 16384 x 7168 136 against 142; with
+// several sums it comes first (4096 x 4096, 8 sums to e4m3: 56 us, 60 behind).
+template <typename T, typename W, int AT_ONCE, int K>
+constexpr bool kLateWeight = sizeof(T) == 2 && K == 2 && (sizeof(W) == 4 || AT_ONCE == 1);
 
 struct Rows {
   const void* p;
@@ -161,6 +169,17 @@ struct Load {
     for (int k = 0; k < K; ++k) raw[k].load(row + part.at[k], part.kStep, part.left[k]);
   }
   __device__ __forceinline__ void get(int k, Pair (&f)[4]) const { raw[k].get(f); }
+};
+
+// The same, loaded where it is used.
+template <typename T, int K>
+struct LateLoad {
+  const T* p[K];
+  __device__ __forceinline__ void load(const T* row, const Part<K, true>& part) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) p[k] = row + part.at[k];
+  }
+  __device__ __forceinline__ void get(int k, Pair (&f)[4]) const { unpack<T>(load_oct(p[k]), f); }
 };
 
 __device__ __forceinline__ void add(Pair (&h)[4], const Pair (&f)[4]) {
@@ -446,15 +465,15 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool
 // than one partial sum.
 //
 // Two octets a thread share the cost of the row's sum: 8192 x 4096 bf16 with
-// residual takes 41.5 us (98 % of the copy bandwidth) against 46 with one octet.
+// residual takes 41.8 us (98 % of the copy bandwidth) against 46 with one octet.
 // Blocks that walk over rows with asynchronous copies ahead took 46.5 there, so a
 // row has a block. With e4m3 output the arithmetic behind the sum, a chain
-// of maximum, scale and conversion, shows: 16384 x 5120 in 105 us, 86 %.
+// of maximum, scale and conversion, shows: 16384 x 5120 in 93 us, 97 %.
 // One row of 8192 takes 2.8 us, most of it the launch.
 // PAIR: a row is shared by the two blocks of a cluster. Their part of it is a
 // multiple of 128 columns, so that no group of columns is in both.
 template <typename T, typename W, bool F8, int AT_ONCE, int K, bool PAIR = false, bool LEAN = false>
-__global__ void __maxnreg__(norm_registers(sizeof(T), sizeof(W), AT_ONCE, K, PAIR, LEAN))
+__global__ void __maxnreg__(norm_registers(sizeof(T), AT_ONCE, K, PAIR, LEAN))
     norm_kernel(const __grid_constant__ FwdArgs a) {
   __shared__ float red[32];
   __shared__ uint32_t top_red[32];
@@ -480,7 +499,7 @@ __global__ void __maxnreg__(norm_registers(sizeof(T), sizeof(W), AT_ONCE, K, PAI
   // AT_ONCE partial sums at a time, with the first of them the residual too.
   constexpr int N = AT_ONCE;
   Load<T, true, K> xv[N], rv;
-  Load<W, true, K> wv;
+  std::conditional_t<kLateWeight<T, W, AT_ONCE, K>, LateLoad<W, K>, Load<W, true, K>> wv;
   Pair h[K][4], f[4];
 #pragma unroll 1
   for (int s0 = 0; s0 < (N > 1 ? a.parts : 1); s0 += N) {
@@ -1083,9 +1102,9 @@ int blocks_by_registers(int threads, int registers) { return 4 * (16384 / (32 * 
 //
 // Of a row in registers, the variant that lets an SM hold two blocks at least
 // (norm_registers; bf16 with residual; "48 -> 40" are registers a thread):
-//  - one sum: 40 registers, which spill a few addresses, only where they hold more
-//    blocks: 4096 x 12288 with e4m3 output 84 -> 63 us, 8192 x 8192 88 -> 79; but
-//    16384 x 5120, where they do not, takes 100 instead of 94.
+//  - one sum: 40 registers only where they hold more blocks: 4096 x 12288 with
+//    e4m3 output 84 -> 63 us, 8192 x 8192 88 -> 79; but 16384 x 5120, where they do
+//    not, took 100 instead of 94.
 //  - several: four at a time, or two where four leave one block (8192 x 8192, 8 sums:
 //    256 -> 226 us) or where there are two (8192 x 7168: 142 -> 92); four in 72
 //    registers for 80 where that holds more (8192 x 7168, 4 sums: 163 -> 117).
@@ -1097,7 +1116,7 @@ int blocks_by_registers(int threads, int registers) { return 4 * (16384 / (32 * 
 //    16384: 99 us, pairs 104); nor fp32 with fewer than three sums (2048 x 12288: 96
 //    us by reading again, pairs 102).
 // Up to a row an SM, one octet a thread is the shortest way.
-Shape shape_fwd(long long rows, int hidden, int es, int ws, int windows, bool vec, int parts, bool by_row, int sms) {
+Shape shape_fwd(long long rows, int hidden, int es, int windows, bool vec, int parts, bool by_row, int sms) {
   Shape s;
   const int octets = int(ceil_div(hidden, 8));
   s.at_once = parts == 1 ? 1 : 4;
@@ -1123,12 +1142,11 @@ Shape shape_fwd(long long rows, int hidden, int es, int ws, int windows, bool ve
     s.half = s.pair ? int(ceil_div(octets, 32)) * 16 * 8 : hidden;
     spread(s, s.half / 8, 2, false);
     const auto fit = [&](int at_once, bool lean) {
-      return blocks_by_registers(s.threads, norm_registers(es, ws, at_once, 2, s.pair, lean));
+      return blocks_by_registers(s.threads, norm_registers(es, at_once, 2, s.pair, lean));
     };
-    const bool narrow = es == 2 && ws == 2;
     if (parts > 1 && es == 2)
-      s.at_once = parts == 2 || s.threads > 512 || (rows > sms && fit(4, narrow) < 2) ? 2 : 4;
-    s.lean = narrow && s.at_once != 2 && fit(s.at_once, true) > fit(s.at_once, false);
+      s.at_once = parts == 2 || s.threads > 512 || (rows > sms && fit(4, true) < 2) ? 2 : 4;
+    s.lean = es == 2 && s.at_once != 2 && fit(s.at_once, true) > fit(s.at_once, false);
     const int blocks = fit(s.at_once, s.lean);
     if (turn == 0 && s.threads <= 1024) alone = blocks * s.threads;
     bool take = s.threads <= 1024 && blocks > (turn == 2 || es == 4 || rows <= sms ? 0 : 1);
@@ -1187,11 +1205,11 @@ RowSplit split_by(long long inner) {
 
 template <typename T, typename W, bool F8, bool PAIR>
 const void* fwd_kernel2(const Shape& s) {
-  if constexpr (sizeof(T) == 2)
+  if constexpr (sizeof(T) == 2) {
     if (s.at_once == 2) return reinterpret_cast<const void*>(norm_kernel<T, W, F8, 2, 2, PAIR>);
-  if constexpr (sizeof(T) == 2 && sizeof(W) == 2)
     if (s.lean) return s.at_once == 4 ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, 4, 2, PAIR, true>)
                                       : reinterpret_cast<const void*>(norm_kernel<T, W, F8, 1, 2, PAIR, true>);
+  }
   return s.at_once == 4 ? reinterpret_cast<const void*>(norm_kernel<T, W, F8, 4, 2, PAIR>)
                         : reinterpret_cast<const void*>(norm_kernel<T, W, F8, 1, 2, PAIR>);
 }
@@ -1336,8 +1354,7 @@ extern "C" int nb_add_rms_norm(const nb_norm_t* a, void* stream, char* err, size
   vec = vec && octets_fit(a->y, 0, 0, f8 ? 1 : es) && (!a->h || octets_fit(a->h, 0, 0, es));
   const int sources = a->parts + (a->residual ? 1 : 0), outputs = a->h ? 2 : 1;
   k.windows = sources > outputs ? sources : outputs;
-  const Shape s =
-      shape_fwd(a->rows, a->hidden, es, size_of(a->weight_dtype), k.windows, vec, a->parts, f8 && !a->group, dev.sms());
+  const Shape s = shape_fwd(a->rows, a->hidden, es, k.windows, vec, a->parts, f8 && !a->group, dev.sms());
   k.half = s.half;
   k.weight = a->weight;
   k.y = a->y;
