@@ -182,6 +182,17 @@ struct LateLoad {
   __device__ __forceinline__ void get(int k, Pair (&f)[4]) const { unpack<T>(load_oct(p[k]), f); }
 };
 
+template <typename T, int K>
+struct LateElements {
+  const T* row;
+  const Part<K, false>& part;
+  __device__ __forceinline__ void get(int k, Pair (&f)[4]) const {
+    Raw<T, false> raw;
+    raw.load(row + part.at[k], part.kStep, part.left[k]);
+    raw.get(f);
+  }
+};
+
 __device__ __forceinline__ void add(Pair (&h)[4], const Pair (&f)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) h[j] = h[j] + f[j];
@@ -541,9 +552,10 @@ __global__ void __maxnreg__(norm_registers(sizeof(T), AT_ONCE, K, PAIR, LEAN))
 // The same for rows off the vector boundary, which go through shared memory:
 // all sources of a row are on their way at once without a register held for
 // them, and single elements come out of shared memory. A row has a warp or a block.
-// Bound by the instructions that single elements take: 8192 x 4097 bf16 in 76 us
-// (single elements straight from memory: 106; octets cut out of the pieces
-// in registers: 142), four fp16 partials of 1013 x 5001 with e4m3 output in 21 us.
+// Bound by the instructions that single elements take: 8192 x 4097 bf16 in 74 us
+// (76 with the weight loaded ahead of the sum; single elements straight from
+// memory: 106; octets cut out of the pieces in registers: 142), four fp16 partials
+// of 1013 x 5001 with e4m3 output in 22 us.
 template <typename T, typename W, bool F8, int K>
 __global__ void __launch_bounds__(kStagedThreads, 2) norm_staged_kernel(const __grid_constant__ FwdArgs a) {
   extern __shared__ uint4 smem[];
@@ -559,8 +571,7 @@ __global__ void __launch_bounds__(kStagedThreads, 2) norm_staged_kernel(const __
     Window<T>::fetch(stage + s * a.window, from.of<T>(a.x[s]), static_cast<const T*>(a.x[s].p), a.hidden, lane, tpr);
   asm volatile("cp.async.commit_group;" ::: "memory");
   const Part<K, false> part(lane, tpr, a.hidden);
-  Load<W, false, K> wv;
-  wv.load(static_cast<const W*>(a.weight), part);
+  const LateElements<W, K> wv{static_cast<const W*>(a.weight), part};
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   row_sync(tpr);
   Pair h[K][4], f[4];
