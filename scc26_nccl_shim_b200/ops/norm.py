@@ -223,7 +223,8 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
     Squares are summed in fp32: rows beyond about 1e19 overflow to y = 0.
 
     `out` gives the outputs' memory (contiguous; `out.h` may be the residual or
-    x_0 itself, nothing else may overlap).
+    x_0 itself, nothing else may overlap). Autograd sees that they were changed: a
+    graph that holds the residual for its backward pass then raises there.
     """
     xs = [x] if isinstance(x, torch.Tensor) else list(x)
     key = (eps, out_dtype, group, _describe(weight), None if residual is None else _describe(residual),
@@ -252,6 +253,10 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
         emu.raw_stream(plan.device), err, _ERR)
     if rc:
         _raise(err, rc)
+    if out is not None:  # autograd has to see that the caller's tensors were changed
+        written = [t for t in (y, scale, None if alone and h is x0 else h, rstd) if t is not None and not t.is_inference()]
+        if written:
+            torch.autograd.graph.increment_version(written)
     return NormOut(y, scale, h, rstd)
 
 

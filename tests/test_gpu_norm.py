@@ -286,6 +286,33 @@ def test_one_source_with_a_copy_of_it(hidden):
     assert same.h is x and torch.equal(same.y, want.y)
 
 
+def test_what_out_overwrites_is_seen_by_autograd():
+    m = norm()
+    res = data((3, 64), torch.float32, 1)
+    x, w = data((3, 64), torch.float32, 2), data((64,), torch.float32, 3)
+    leaf = data((3, 64), torch.float32, 4).requires_grad_()
+    loss = (leaf * res).sum()  # holds res for its gradient
+    out = m.NormOut(torch.empty_like(x), None, res, torch.empty(3, device=DEV))
+    before = [t._version for t in (out.y, res, out.rstd, x)]
+    m.add_rms_norm(x, w, res, out=out)
+    assert [t._version > v for t, v in zip((out.y, res, out.rstd, x), before)] == [True, True, True, False]
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    # e4m3 with scales; a single x that comes back as h itself is not written
+    out = m.NormOut(torch.empty(3, 64, dtype=E4M3, device=DEV), torch.empty(3, 1, device=DEV), x,
+                    torch.empty(3, device=DEV))
+    written = (out.y, out.scale, out.rstd)
+    before = [t._version for t in (*written, x)]
+    m.add_rms_norm(x, w, out_dtype=E4M3, out=out)
+    assert [t._version > v for t, v in zip((*written, x), before)] == [True, True, True, False]
+    with torch.inference_mode():  # tensors of that mode have no version
+        free = m.NormOut(torch.empty_like(x), None, torch.empty_like(x), torch.empty(3, device=DEV))
+        m.add_rms_norm(x, w, res, out=free)
+        before = res._version
+        m.add_rms_norm(x, w, res, out=m.NormOut(free.y, None, res, free.rstd))
+        assert res._version > before
+
+
 # ------------------------------------------------------------------ gradient
 
 def grad_reference(dy, h, w, rstd, dh):
