@@ -148,8 +148,9 @@ class GradNorm(_Bound):
         """fp32 [norm, coefficient] on the device: norm = scale * the gradients'
         norm, coefficient = scale * min(1, max_norm / (norm + 1e-6)), what the
         gradients are to be multiplied with (AdamW.step takes it as its scale).
-        Where the norm is not finite the coefficient is NaN. The same inputs give
-        the same bits."""
+        Where the norm is not finite the coefficient is NaN; a norm above 2^126
+        (before the scale) counts as infinite, since fp32 has no normal number for its
+        reciprocal. The same inputs give the same bits."""
         self._check_storages()
         out = torch.empty_strided((2,), (1,), dtype=torch.float32, device=self.device)
         ws = torch.empty_strided((self._partials,), (1,), dtype=torch.float64, device=self.device)

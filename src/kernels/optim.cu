@@ -29,6 +29,7 @@
 #include <cstring>
 #include <memory>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "core/tensor_table.h"
@@ -45,6 +46,7 @@ constexpr int kThreads = 256;
 constexpr unsigned kChunk = kThreads * 8;         // AdamW: eight elements per thread
 constexpr int kNormOctets = 4;                    // the norm: four times that, all loaded before the first is used
 constexpr unsigned kNormChunk = kChunk * kNormOctets;
+constexpr float kLargest = 3.4028235e38f;         // finite in fp32
 static_assert(NB_OPTIM_BLOCK == 256, "a block is one warp's elements");
 
 // One tensor of the work list; its gradients' addresses follow the entries.
@@ -346,7 +348,7 @@ template <typename P, typename C, typename G, bool S8, int WORDS>
 __global__ void __launch_bounds__(kThreads, S8 ? 4 : 3) adamw_kernel(const __grid_constant__ AdamArgs<WORDS> a) {
   float scale = a.s.scale_host;
   if (a.s.scale) scale *= *a.s.scale;
-  if (!(fabsf(scale) <= 3.4028235e38f)) return;  // no step
+  if (!(fabsf(scale) <= kLargest)) return;  // no step
   float lr = a.s.lr_host, root = a.s.t_root, size = a.s.t_lr_m;
   unsigned t = a.s.t_host;
   if (a.s.t || a.s.lr) {
@@ -419,8 +421,13 @@ struct NormRaw<G, false> {
   }
 };
 
+constexpr uint32_t kLeastSum = (127u - 120u) << 23;  // 2^-120 as an integer
+
 // Squares of eight elements are added in fp32 and those sums in fp64: the
-// result does not depend on how many elements there are.
+// result does not depend on how many elements there are. Where fp32 does not
+// hold the squares they are formed again in fp64: above its range, or with a sum
+// below 2^-120 (each is off by 2^-150 at most, together by less than 2^-27 of a larger
+// sum). The sums of fp16 gradients are never there, unless they are zero.
 template <typename G, int WORDS>
 __global__ void __launch_bounds__(kThreads, 4) grad_norm_kernel(const __grid_constant__ GradArgs<WORDS> a) {
   __shared__ double sums[kThreads / 32];
@@ -455,12 +462,31 @@ __global__ void __launch_bounds__(kThreads, 4) grad_norm_kernel(const __grid_con
           for (int j = 0; j < 8; ++j) g[u][j] += f[j];
         }
       }
+      float s[kNormOctets] = {};
+      uint32_t off = 0;  // as integers, so that a NaN is above all
 #pragma unroll
       for (int u = 0; u < kNormOctets; ++u) {
-        float s = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s = fmaf(g[u][j], g[u][j], s);
-        total += double(s);
+        for (int j = 0; j < 8; ++j) s[u] = fmaf(g[u][j], g[u][j], s[u]);
+        off = max(off, __float_as_uint(s[u]) - kLeastSum);
+      }
+      if (std::is_same_v<G, __half> || __builtin_expect(off < 0x7f800000u - kLeastSum, 1)) {
+#pragma unroll
+        for (int u = 0; u < kNormOctets; ++u) total += double(s[u]);
+      } else {
+        uint32_t any = 0;
+#pragma unroll
+        for (int u = 0; u < kNormOctets; ++u)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) any |= __float_as_uint(g[u][j]);
+        if (!(any << 1)) return;  // zeros: nothing to add (with it 200 M bf16 zeros took 74 us, not 63)
+#pragma unroll
+        for (int u = 0; u < kNormOctets; ++u) {
+          double wide = 0.0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) wide = ::fma(double(g[u][j]), double(g[u][j]), wide);
+          total += wide;
+        }
       }
     };
     if (e.vec && left >= 256 * kNormOctets) add(NormRaw<G, true>());
@@ -488,11 +514,12 @@ __global__ void __launch_bounds__(1024) grad_norm_end_kernel(const double* parti
   if (threadIdx.x < 32) {
     s = warp_sum(sums[threadIdx.x]);
     if (threadIdx.x == 0) {
-      const double norm = scale * sqrt(s);
+      // Above 2^126 the reciprocal of the norm is no normal fp32 number: an overflow.
+      const double root = sqrt(s), norm = scale * (root > 0x1p126 ? HUGE_VAL : root);
       const float shown = float(norm);
       const double clip = max_norm / (norm + 1e-6);
       out[0] = shown;
-      out[1] = fabsf(shown) <= 3.4028235e38f ? float(scale * (clip < 1.0 ? clip : 1.0)) : __int_as_float(0x7fffffff);
+      out[1] = fabsf(shown) <= kLargest ? float(scale * (clip < 1.0 ? clip : 1.0)) : __int_as_float(0x7fffffff);
     }
   }
 }

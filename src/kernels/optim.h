@@ -59,7 +59,8 @@ void* nb_grad_norm_create(int device, int count, int parts, int dtype, const uin
 // Doubles of workspace for one call.
 int nb_grad_norm_partials(const void* handle);
 // out[0] = scale * sqrt(sum of squares), out[1] = scale * min(1, max_norm / (out[0] + 1e-6)), or
-// NaN where out[0] is not finite (a step that takes it as its scale is skipped).
+// NaN where out[0] is not finite (a step that takes it as its scale is skipped). A root above
+// 2^126 counts as infinite.
 int nb_grad_norm(const void* handle, double max_norm, double scale, float* out, double* workspace, void* stream,
                  char* err, size_t errcap);
 void nb_grad_norm_destroy(void* handle);

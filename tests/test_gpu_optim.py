@@ -373,6 +373,60 @@ def test_a_step_is_skipped_after_an_overflow():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("parts", [1, 3])
+@pytest.mark.parametrize("size", [1e-39, 1e-30, 1e-22, 1e-19, 6e18, 1e20, 1e30, 1e35])
+def test_grad_norm_where_squares_leave_fp32(dtype, parts, size):
+    m = optim()
+    for at in (0, 1):
+        grads = [[data(n + 1, dtype, 10 * k + n, size)[at:at + n] for k in range(parts)] for n in (5, 2048, 5003)]
+        f = m.GradNorm(grads)
+        total = sum(gradient(g, 1.0)[0].square().sum() for g in grads)
+        slack = sum((2 * gradient(g, 1.0)[0].abs() * gradient(g, 1.0)[1]).sum() for g in grads)
+        ref = total.sqrt()
+        # eight squares (9 u), the result rounded (u, or half of 2^-149)
+        tol = ref * 16 * U + slack / (2 * ref) + 2.0 ** -149
+        for max_norm, scale in ((1.0, 1.0), (float(ref) / 2, 1.0), (1.0, 0.25)):
+            out = f(max_norm, scale).double()
+            assert abs(out[0] - scale * ref) <= scale * tol + 2.0 ** -149
+            coef = scale * min(1.0, max_norm / (scale * float(ref) + 1e-6))
+            assert abs(out[1] - coef) <= coef * (4 * U + float(tol / ref)) + 2.0 ** -149
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_grad_norm_of_one_large_or_small_element(dtype):
+    m = optim()
+    for big in (3e18, 2e19, 1e25, 8e37):  # beside 5000 of about 1, and 5000 of nothing
+        g = data(5000, dtype, 1)
+        g[4321] = big
+        out = m.GradNorm([g, torch.zeros(5000, dtype=dtype, device=DEV)])(1.0).double()
+        ref = float(g[4321].double())
+        assert abs(out[0] - ref) <= ref * 16 * U and abs(out[1] - 1 / ref) <= 16 * U / ref
+    g = torch.zeros(5000, dtype=dtype, device=DEV)
+    assert m.GradNorm([g])(1.0).tolist() == [0.0, 1.0]
+    g[4321] = 2.0 ** -120
+    assert m.GradNorm([g])(1.0).tolist() == [2.0 ** -120, 1.0]
+    # From 2^126 on, 1 / norm is no normal number: an overflow.
+    g[4321] = 2.0 ** 126
+    out = m.GradNorm([g])(1.0)
+    assert float(out[0]) == 2.0 ** 126 and float(out[1]) == 2.0 ** -126
+    g[1] = 2.0 ** 126
+    out = m.GradNorm([g])(1.0)
+    assert out[0].isinf() and out[1].isnan()
+
+
+def test_a_step_is_clipped_not_skipped_after_a_large_gradient():
+    m = optim()
+    for state in ("float32", "8bit"):
+        p, g = data(5000, torch.float32, 1), data(5000, torch.float32, 2)
+        g[17] = 1e20
+        opt, before = m.AdamW([p], [g], state=state, weight_decay=0.0), p.clone()
+        opt.step(1, LR, scale=m.GradNorm([g])(1.0)[1])
+        # g[17] is scaled to 1 - 1e-13: the first step's update is lr g / (|g| + eps)
+        assert abs(float(before[17] - p[17]) - LR) <= 32 * U * LR + 4 * U * abs(float(before[17]))
+        assert p.isfinite().all() and all(x.isfinite().all() for x in opt.moments(0))
+
+
 # ------------------------------------------------------------------ use
 
 def test_device_scalars_and_graphs():
