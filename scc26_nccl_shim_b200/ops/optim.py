@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import itertools
 import math
 import weakref
 from typing import Sequence
@@ -25,6 +26,7 @@ E4M3 = torch.float8_e4m3fn
 NCCL_E4M3 = 10
 BLOCK = 256  # elements that share a scale in the 8-bit states
 _ERR = emu.ERR.size
+_data_ptr, _storage_ptr = torch.Tensor.data_ptr, torch.UntypedStorage.data_ptr
 
 
 class _Desc(C.Structure):  # nb_adamw_t
@@ -94,8 +96,8 @@ def _check_overlap(written: Sequence[torch.Tensor], read: Sequence[torch.Tensor]
 
 
 class _Bound:
-    """The tensors that a handle points to: held alive, and refused if their
-    storage was moved since."""
+    """The tensors that a handle points to: their memory is held alive, and
+    refused if a storage was resized or moved since."""
 
     def __init__(self, device: torch.device, tensors: Sequence[torch.Tensor]):
         if device.type != "cuda":
@@ -114,7 +116,7 @@ class _Bound:
         raise TypeError(f"{type(self).__name__} is bound to its tensors: make a new one instead of copying it")
 
     def _check_storages(self) -> None:
-        if [s.data_ptr() for s in self._storages] != self._where:
+        if [*map(_storage_ptr, self._storages)] != self._where:
             raise RuntimeError("a tensor's storage was resized or moved since this was made")
 
 
@@ -122,7 +124,9 @@ class GradNorm(_Bound):
     """The L2 norm of many gradients, as if they were one vector.
 
     `grads`: tensors (fp16, bf16 or fp32, one type, contiguous, any shapes), or
-    for each gradient a sequence of 1 to 8 partial ones that are added first.
+    for each gradient a sequence of 1 to 8 partial ones that are added first. They are
+    bound by their memory: a gradient that is replaced (by a backward pass after
+    `zero_grad(set_to_none=True)`, torch's default) is not seen, the old one is read.
     """
 
     def __init__(self, grads):
@@ -181,8 +185,13 @@ class AdamW(_Bound):
     GradNorm's coefficient, which skips such a step. `states=(exp_avg,
     exp_avg_sq)` takes given ones instead of zeros (to resume).
 
-    The tensors are bound by their memory: give new ones (after `.data =` or a
-    resize) to a new AdamW. No two of them may overlap where one is written.
+    The tensors are bound by their memory: give new ones to a new AdamW. A step
+    refuses a storage that was resized; and it looks at one parameter and its copy, the
+    next step at the next ones, and refuses if they were given other memory (`.data =`,
+    Module.to). It cannot see that a gradient was replaced: after
+    `zero_grad(set_to_none=True)`, torch's default, a backward pass makes new ones and
+    the step would read the old; zero the bound ones in place (set_to_none=False).
+    No two tensors may overlap where one is written.
     """
 
     def __init__(self, params, grads, *, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01,
@@ -247,6 +256,10 @@ class AdamW(_Bound):
         flat = [t for g in parts for t in g]
         _check_overlap(written, flat)
         super().__init__(device, written + flat)
+        # Whether a tensor still has its memory: a look at 64 would take 4 of a step's 13 us, so a
+        # step looks at one parameter (and its copy), the next step at the next.
+        owned = zip(params, copies) if copies else zip(params)
+        self._looks = itertools.cycle([(ts, [t.data_ptr() for t in ts]) for ts in owned])
         # Autograd has to see that parameters were changed.
         self._versions = [t for t in params + (copies or []) if not t.is_inference()]
         tables = [(C.c_uint64 * len(params))(*sizes), _addresses(params), _addresses(copies) if copies else None,
@@ -283,6 +296,9 @@ class AdamW(_Bound):
         replayed with new ones. A device scale that is not finite (GradNorm's
         coefficient after an overflow) leaves parameters and states as they were."""
         self._check_storages()
+        tensors, addresses = next(self._looks)
+        if [*map(_data_ptr, tensors)] != addresses:
+            raise RuntimeError("a parameter or its copy was moved to other memory since this was made")
         t, t_dev = self._scalar(t, "t", torch.int64)
         lr, lr_dev = self._scalar(lr, "lr", torch.float32)
         scale, scale_dev = self._scalar(scale, "scale", torch.float32)

@@ -557,3 +557,33 @@ def test_offsets_beyond_32_bits():
     got = p[-6000:].double()
     assert ((got - want).abs() <= half_step(want, torch.bfloat16) * 1.001 + want.abs() * 32 * U).all()
     assert not p[:-6000].any()
+
+
+def test_parameters_and_copies_given_other_memory_are_refused():
+    m = optim()
+    for which in (0, 1):
+        p, g = data(100, torch.float32, 1).requires_grad_(), data(100, torch.float32, 2)
+        copy = p.detach().bfloat16()
+        opt = m.AdamW([p], [g], copies=[copy])
+        opt.step(1, LR)
+        t = (p, copy)[which]
+        home, held = t.data, [x.clone() for x in (p, opt.exp_avg[0])]
+        t.data = t.data.clone()
+        with pytest.raises(RuntimeError, match="moved"):
+            opt.step(2, LR)
+        assert all(torch.equal(a, b) for a, b in zip((p, opt.exp_avg[0]), held))
+        t.data = home
+        opt.step(2, LR)
+
+
+def test_one_of_many_parameters_given_other_memory_is_refused():
+    """Each step looks at the next one."""
+    m = optim()
+    p = [data(100, torch.float32, k) for k in range(41)]
+    opt = m.AdamW(p, [data(100, torch.float32, 50)] * 41)
+    for t in range(1, 24):
+        opt.step(t, LR)
+    p[33].data = p[33].clone()
+    with pytest.raises(RuntimeError, match="moved"):
+        for t in range(24, 24 + 41):
+            opt.step(t, LR)
