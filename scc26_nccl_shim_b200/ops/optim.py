@@ -294,7 +294,8 @@ class AdamW(_Bound):
         with `scale`. Each may be a one-element tensor on the device (t int64, the
         others fp32), read when the kernel runs, so that a captured step can be
         replayed with new ones. A device scale that is not finite (GradNorm's
-        coefficient after an overflow) leaves parameters and states as they were."""
+        coefficient after an overflow), or a device lr that is not, leaves parameters and
+        states as they were; a device t below 1 counts as 1."""
         self._check_storages()
         tensors, addresses = next(self._looks)
         if [*map(_data_ptr, tensors)] != addresses:

@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, S8 ? 4 : 3) adamw_kernel(const __gri
       root = 1.0f / sqrtf(-expm1f(float(td) * a.ln_b2));
     }
     size = lr * inv1;
+    if (!(fabsf(size) <= kLargest)) return;  // as the host refuses such a step
   }
   const StepValues r{scale, lr, size, root, t};
   const Entry* entries = reinterpret_cast<const Entry*>(a.words);

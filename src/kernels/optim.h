@@ -48,8 +48,8 @@ struct nb_adamw_t {
 void* nb_adamw_create(const nb_adamw_t* a, char* err, size_t errcap);
 // Step number t >= 1, learning rate and gradient scale; each may instead be
 // read on the device (t_dev: int64, the others float), and the device's scale
-// multiplies `scale`. A scale that is not finite when the kernel runs leaves
-// every tensor as it was.
+// multiplies `scale`. A scale, or an lr / (1 - beta1^t), that is not finite when
+// the kernel runs leaves every tensor as it was; t below 1 on the device counts as 1.
 int nb_adamw_step(const void* handle, int64_t t, const int64_t* t_dev, double lr, const float* lr_dev, double scale,
                   const float* scale_dev, void* stream, char* err, size_t errcap);
 void nb_adamw_destroy(void* handle);

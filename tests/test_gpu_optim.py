@@ -427,6 +427,27 @@ def test_a_step_is_clipped_not_skipped_after_a_large_gradient():
         assert p.isfinite().all() and all(x.isfinite().all() for x in opt.moments(0))
 
 
+@pytest.mark.parametrize("state", ["float32", "8bit"])
+def test_a_device_lr_that_is_not_finite_changes_nothing(state):
+    m = optim()
+    p, g = data(5000, torch.float32, 1), data(5000, torch.float32, 2)
+    copy = p.bfloat16()
+    opt = m.AdamW([p], [g], state=state, copies=[copy])
+    lr, t = torch.full((1,), LR, device=DEV), torch.ones(1, dtype=torch.int64, device=DEV)
+    opt.step(1, lr)
+    kept = [p.clone(), copy.clone(), *[x.clone() for x in opt.moments(0)]]
+    for bad in (math.nan, math.inf, -math.inf, 2e38):  # 2e38 / (1 - 0.9) is not finite
+        lr.fill_(bad)
+        opt.step(1, lr)
+        opt.step(t, lr)
+    opt.step(t, 2e38)
+    for a, b in zip(kept, [p, copy, *opt.moments(0)]):
+        assert torch.equal(a, b)
+    lr.fill_(LR)
+    opt.step(2, lr)
+    assert not torch.equal(kept[0], p) and p.isfinite().all()
+
+
 # ------------------------------------------------------------------ use
 
 def test_device_scalars_and_graphs():
