@@ -270,6 +270,7 @@ class AdamW(_Bound):
                      DTYPE[ctype] if ctype else 0, NCCL_E4M3 if self._eight else DTYPE[torch.float32],
                      seed & 0xFFFFFFFF, *[C.cast(t, C.c_void_p) if t is not None else None for t in tables], b1, b2, eps)
         err = emu.ERR.buf
+        self._step = lib().nb_adamw_step
         self._handle = lib().nb_adamw_create(C.byref(desc), err, _ERR)
         if not self._handle:
             raise RuntimeError(err.value.decode())
@@ -304,7 +305,7 @@ class AdamW(_Bound):
         lr, lr_dev = self._scalar(lr, "lr", torch.float32)
         scale, scale_dev = self._scalar(scale, "scale", torch.float32)
         err = emu.ERR.buf
-        rc = lib().nb_adamw_step(self._handle, t, t_dev, lr, lr_dev, scale, scale_dev, emu.raw_stream(self._index), err, _ERR)
+        rc = self._step(self._handle, t, t_dev, lr, lr_dev, scale, scale_dev, emu.raw_stream(self._index), err, _ERR)
         if rc:
             raise (ValueError if rc == -1 else RuntimeError)(f"{err.value.decode()} ({rc})")
         if self._versions:
