@@ -14,8 +14,11 @@ inline void op_message(char* err, size_t cap, const char* msg) {
   if (err && cap) std::snprintf(err, cap, "%s", msg);
 }
 
+// `code` above 0: a CUDA error, which is reported here and must not come up again as the
+// last error of a later launch of the caller's.
 inline int op_refuse(char* err, size_t cap, const char* msg, int code = -1) {
   op_message(err, cap, msg);
+  if (code > 0) cudaGetLastError();
   return code;
 }
 
@@ -39,6 +42,7 @@ class OpDevice {
     }
   }
   ~OpDevice() {
+    if (err_ != cudaSuccess) cudaGetLastError();  // the call reports it
     if (switched_) cudaSetDevice(before_);
   }
   OpDevice(const OpDevice&) = delete;

@@ -9,6 +9,8 @@ of each stored type:
   it is off by less than 2^-17 of itself; rstd by half that plus what the
   sum's own error moves it; the products after it add a few u: 2^-16 covers all.
 """
+import ctypes as C
+
 import pytest
 import torch
 
@@ -446,3 +448,22 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(dx[-4:], tx) and not dx[:-4].any()
     # four rows that are not zero, in another grouping: fp32 sums of four terms
     assert ((dw.double() - tw.double()).abs() <= tw.double().abs() * 2.0 ** -7 + 1e-6).all()
+
+
+def test_a_device_that_is_not_there_leaves_no_error_behind():
+    """The refused call returns its code; torch, which looks at CUDA's last error after its own launches, finds none."""
+    m = norm()
+    from scc26_nccl_shim_b200.ops import optim
+    x, w = data((4, 64), torch.bfloat16, 1), data((64,), torch.bfloat16, 2)
+    y, rstd, err = torch.empty_like(x), torch.empty(4, device=DEV), C.create_string_buffer(256)
+    p, missing = x.data_ptr(), 60
+    call = m._FWD[1].pack(p, 64, 0, 0, 0, 0, w.data_ptr(), y.data_ptr(), 0, 0, rstd.data_ptr(), 4, 1, missing, 64, 1, 9, 9,
+                          9, 0, 1e-6)
+    assert m.lib().nb_add_rms_norm(call, None, err, 256) > 0 and b"device" in err.value
+    torch.zeros(8, device=DEV)
+    assert m.lib().nb_add_rms_norm_backward_workspace(missing, 4, 64, 9) == 0
+    torch.zeros(8, device=DEV)
+    one, at = (C.c_uint64 * 1)(4), (C.c_uint64 * 1)(p)
+    assert optim.lib().nb_grad_norm_create(missing, 1, 1, 9, one, at, err, 256) is None and b"device" in err.value
+    torch.zeros(8, device=DEV)
+    assert torch.cuda.current_device() == 0
