@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import operator
 import struct
 from typing import NamedTuple, Sequence
 
@@ -123,6 +124,13 @@ def _check_weight(weight: torch.Tensor, hidden: int, dtype: torch.dtype, device:
     return DTYPE[weight.dtype]
 
 
+def _integer(n, name: str) -> int:
+    try:
+        return operator.index(n)
+    except TypeError:
+        raise TypeError(f"{name}: expected an integer, got {n!r}") from None
+
+
 def _like(t: torch.Tensor, ref: torch.Tensor, name: str) -> None:
     if t.dtype != ref.dtype:
         raise TypeError(f"{name}: expected {ref.dtype}, got {t.dtype}")
@@ -227,6 +235,8 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
     graph that holds the residual for its backward pass then raises there.
     """
     xs = [x] if isinstance(x, torch.Tensor) else list(x)
+    if type(group) is not int:  # 32.0 would be the same key as 32
+        group = _integer(group, "group")
     key = (eps, out_dtype, group, _describe(weight), None if residual is None else _describe(residual),
            *[_describe(t) for t in xs])
     plan = _plans.get(key) or _keep(key, _plan_forward(xs, weight, residual, eps, out_dtype, group))

@@ -136,6 +136,16 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+@pytest.mark.parametrize("group", [32.0, 64.0, "32"])
+def test_norm_refuses_a_group_that_is_not_an_integer(group):
+    """And what it refuses is not kept: 32 == 32.0, so that both would be one combination of types and shapes."""
+    for g in (group, group):
+        with pytest.raises((TypeError, ValueError), match="group"):
+            norm.add_rms_norm(x(4, 64), W, out_dtype=E4M3, group=g)
+    with pytest.raises(ValueError, match="CUDA"):
+        norm.add_rms_norm(x(4, 64), W, out_dtype=E4M3, group=int(float(group)))
+
+
 @pytest.mark.parametrize("eps", [1e-50, 1e-42, 1e39, -1e-6, float("inf")])
 def test_norm_refuses_an_eps_beyond_fp32(eps):
     with pytest.raises(ValueError, match="eps"):
