@@ -611,12 +611,13 @@ __device__ __forceinline__ void sum8(const FwdArgs& a, const Row& from, const Pa
 }
 
 // The turns that a block of kLongThreads takes over a long row: turn k is the
-// k-th eight elements of its threads. Whole warps take every turn.
+// k-th eight elements of its threads. Whole warps take every turn; a thread without
+// elements in one gets the row's first place and left <= 0.
 template <bool VEC, typename F>
 __device__ __forceinline__ void each_turn(int hidden, F f) {
   const int turns = (hidden + 8 * kLongThreads - 1) / (8 * kLongThreads);
   Part<1, VEC> part(threadIdx.x, kLongThreads, hidden);
-  const int first = part.at[0];  // 0 too for a thread without elements in a row below one turn
+  const int first = VEC ? int(threadIdx.x) * 8 : part.at[0];
   for (int k = 0; k < turns; ++k) {
     part.at[0] = first + k * 8 * kLongThreads;
     part.left[0] = hidden - part.at[0];

@@ -315,6 +315,16 @@ def test_what_out_overwrites_is_seen_by_autograd():
         assert res._version > before
 
 
+@pytest.mark.parametrize("hidden", [301, 511])
+def test_short_rows_of_many_sources(hidden):
+    """More of them than shared memory holds for a block of rows: fp32 rows off the boundary, read again in each pass."""
+    m = norm()
+    xs = [data((37, hidden), torch.float32, k) for k in range(8)]
+    res, w = data((37, hidden), torch.float32, 8), data((hidden,), torch.float32, 9)
+    for out_dtype, group in ((None, 0), (E4M3, 0), (E4M3, 64)):
+        check(m.add_rms_norm(xs, w, res, out_dtype=out_dtype, group=group), xs, w, res, 1e-6, group)
+
+
 # ------------------------------------------------------------------ gradient
 
 def grad_reference(dy, h, w, rstd, dh):
