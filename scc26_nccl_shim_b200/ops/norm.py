@@ -221,7 +221,8 @@ def add_rms_norm(x, weight: torch.Tensor, residual: torch.Tensor | None = None, 
     sums, added in order in fp32); fp16, bf16 or fp32, rows at up to two
     strides. `weight` [hidden] has x's type or fp32. y is computed from the fp32
     sum and rounded once; `h` is the sum rounded to x's type. A single x without
-    a residual comes back as `h` itself.
+    a residual comes back as `h` itself. Nothing is recorded by autograd, whether inputs
+    require gradients or not: call add_rms_norm_backward.
 
     `out_dtype=torch.float8_e4m3fn`: y in e4m3, round to nearest even, with fp32
     scales [..., ceil(hidden / group)] (`group` 32, 64 or 128 columns) or
@@ -325,8 +326,10 @@ def add_rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
     dx = rstd * (dy * w - n * mean(dy * w * n)) + dh with n = h * rstd is the
     gradient of every partial sum and of the residual; `dh` is the gradient that
     reaches the sum on its other way (the residual stream). dweight = sum over
-    rows of dy * n, in the weight's type, added in an order that depends on
-    the sizes alone. `h` and `rstd` are add_rms_norm's; dy, h and dh have one type.
+    rows of dy * n, in the weight's type, added without atomics: the same values give the
+    same bits as long as the sizes, types, strides and alignment of the tensors and the
+    number of the GPU's SMs are the same (another of them may take another kernel, or other
+    blocks). `h` and `rstd` are add_rms_norm's; dy, h and dh have one type.
     """
     key = (_describe(dy), _describe(h), _describe(weight), _describe(rstd), None if dh is None else _describe(dh))
     plan = _plans.get(key) or _keep(key, _plan_backward(dy, h, weight, rstd, dh))

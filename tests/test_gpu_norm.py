@@ -477,3 +477,22 @@ def test_a_device_that_is_not_there_leaves_no_error_behind():
     assert optim.lib().nb_grad_norm_create(missing, 1, 1, 9, one, at, err, 256) is None and b"device" in err.value
     torch.zeros(8, device=DEV)
     assert torch.cuda.current_device() == 0
+
+
+@pytest.mark.parametrize("rows, hidden", [(3, 64), (300, 1000), (70, 4096), (5, 9000)])
+def test_gradient_at_two_alignments(rows, hidden):
+    """The same values at another offset take another kernel: dweight is added in another order, within the same bound."""
+    m = norm()
+    w = data((hidden,), torch.float32, 3)
+    h, dy = data((rows, hidden), torch.bfloat16, 1, 2.0), data((rows, hidden), torch.bfloat16, 2)
+    rstd = (h.double().square().mean(-1) + 1e-6).rsqrt().float()
+    rx, tx, rw, tw = grad_reference(dy, h, w, rstd, None)
+    flat = torch.empty(2, rows * hidden + 1, dtype=torch.bfloat16, device=DEV)
+    for t, v in zip(flat, (dy, h)):
+        t[1:].copy_(v.view(-1))
+    for d, hh in ((dy, h), [t[1:].view(rows, hidden) for t in flat]):
+        dx, dw = m.add_rms_norm_backward(d, hh, w, rstd)
+        assert ((dx.double() - rx).abs() <= half_step(rx, torch.bfloat16) * 1.001 + tx).all()
+        assert ((dw.double() - rw).abs() <= half_step(rw, torch.float32) * 1.001 + tw).all()
+        again = m.add_rms_norm_backward(d, hh, w, rstd)
+        assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
