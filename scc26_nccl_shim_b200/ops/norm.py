@@ -1,8 +1,8 @@
 """Root-mean-square norm of a sum: what follows an AllReduce of activations.
 
-The partial sums of a row-parallel product (one tensor per rank, 1 to 8 of
-them) and the residual are added and normalised in one pass, with the result
-in the input's type or in e4m3 with scales; and the gradient of that.
+The partial sums of a row-parallel product (1 to 8 tensors of one GPU; after a
+collective its one sum) and the residual are added and normalised in one pass, with
+the result in the input's type or in e4m3 with scales; and the gradient of that.
 
 The kernels run on the current stream of the tensors' device, whichever device
 is current, and can be captured into a CUDA graph. Gradients are computed by

@@ -5,7 +5,7 @@ Both are bound to their tensors once (an optimizer's parameters, gradient
 buckets and states stay where they are), then run with a launch or two per
 call on the current stream of their device, whichever device is current; calls
 can be captured into a CUDA graph. A gradient may be given as 1 to 8 partial
-ones (per rank or per micro-batch), added in order in fp32.
+ones of that device (of micro-batches, or of ranks that share it), added in order in fp32.
 """
 from __future__ import annotations
 
@@ -180,10 +180,16 @@ class AdamW(_Bound):
     `state="float32"`: `exp_avg`, `exp_avg_sq` are fp32 tensors. `state="8bit"`:
     they are pairs (e4m3 codes, fp32 scale per block of 256 elements), of m and
     of sqrt(v), rounded at random with bits that are a hash of (`seed`, t, tensor,
-    element); `moments(i)` gives their values. A gradient that is not finite
-    spoils the states of its block, as one of its element in fp32: clip with
-    GradNorm's coefficient, which skips such a step. `states=(exp_avg,
-    exp_avg_sq)` takes given ones instead of zeros (to resume).
+    element); `moments(i)` gives their values. The mean of m and of sqrt(v) is kept; v
+    itself is 5 % high on average at beta2 = 0.999, and a single one between 0.6 and
+    1.7 times the exact v (5th to 95th percentile, simulated with gradients of one distribution;
+    2.5 %, 0.7 and 1.5 at 0.95). `states=(exp_avg, exp_avg_sq)` takes given ones instead of
+    zeros (to resume).
+
+    A gradient (times `scale`) that is not finite, or beyond 1.8e19, whose square fp32 does not
+    hold, spoils the states of its block in 8 bits, of its element in fp32: clip with
+    GradNorm's coefficient, which brings large ones down and skips a step with one that is
+    not finite.
 
     The tensors are bound by their memory: give new ones to a new AdamW. A step
     refuses a storage that was resized; and it looks at one parameter and its copy, the

@@ -2,7 +2,7 @@
 //
 // These entry points have no counterpart in the reference: they are the work
 // that follows a ReduceScatter or AllReduce of gradients. A gradient may be
-// given as 1 to 8 partial ones (per rank or per micro-batch), which the
+// given as 1 to 8 partial ones in the device's memory (per micro-batch or rank), which the
 // kernels add in order, in fp32, as the collectives fold them.
 //
 // A handle describes tensors of one device; it holds their addresses, not the

@@ -472,8 +472,8 @@ __device__ __forceinline__ void finish_row(const FwdArgs& a, long long row, bool
 
 // One row per tpr threads, in registers: every load is issued before the
 // first value is used, and a row's threads meet once (twice with one e4m3
-// scale per row). Octets on their boundary. W: the weight's type; MANY: more
-// than one partial sum.
+// scale per row). Octets on their boundary. W: the weight's type; AT_ONCE:
+// partial sums whose loads are issued together.
 //
 // Two octets a thread share the cost of the row's sum: 8192 x 4096 bf16 with
 // residual takes 41.8 us (98 % of the copy bandwidth) against 46 with one octet.

@@ -1,5 +1,5 @@
 // Root-mean-square norm of a sum: the partial sums of a row-parallel product
-// (one per rank, in rank order) plus the residual, with the normalised row in
+// (in one device's memory, in rank order) plus the residual, with the normalised row in
 // the input's type or in e4m3 with scales; and its gradient.
 //
 // These entry points have no counterpart in the reference: they are the work
